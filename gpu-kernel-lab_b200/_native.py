@@ -8,6 +8,7 @@ if the library is missing or the device is not an sm_100 GPU the call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -21,6 +22,7 @@ KL_DT_BF16, KL_DT_F16, KL_DT_F32 = 0, 1, 2
 KL_W8_ROW, KL_W8_GROUP, KL_W4_SYM, KL_W4_ASYM, KL_BF16_DENSE = range(5)
 KL_FLAG_FORCE_SIMT, KL_FLAG_FORCE_TC, KL_FLAG_PDL, KL_FLAG_Y_TRANSPOSED, KL_FLAG_PERSISTENT = 1, 2, 4, 8, 16
 KL_GROUPED_INT8_MMA = 1
+KL_KV_SAME, KL_KV_INT8 = 0, 1
 
 EXPORTED_SYMBOLS = (
     "kl_linear", "kl_linear_workspace_bytes", "kl_project", "kl_int4_gemv",
@@ -30,6 +32,7 @@ EXPORTED_SYMBOLS = (
     "kl_grouped_table_bytes", "kl_grouped_encode", "kl_grouped_workspace_bytes", "kl_linear_grouped",
     "kl_linear_noalloc", "kl_topk_rows_workspace_bytes", "kl_topk_rows", "kl_topk_merge_rows", "kl_rmsnorm",
     "kl_linear_topk", "kl_linear_topk_workspace_bytes", "kl_grouped_digits_bytes", "kl_grouped_encode_ex",
+    "kl_qk_norm_rope_write", "kl_read_kv", "kl_paged_attention", "kl_paged_attention_workspace_bytes",
 )
 
 
@@ -39,7 +42,10 @@ class KlProblem(ctypes.Structure):
                 ("zeros", ctypes.c_void_p), ("y", ctypes.c_void_p), ("m", ctypes.c_int), ("n", ctypes.c_int),
                 ("k", ctypes.c_int), ("group", ctypes.c_int)]
 
-_P, _I, _S = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+#: ``kl_kv_cache`` of include/kl_b200.h, packed into bytes: four pointers, six strides, five ints
+KV_CACHE = struct.Struct("@4P6q5i4x")
+
+_P, _I, _S, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong
 _SIGNATURES = {
     "kl_linear": (_I, [_P, _I, _I, _I, _P, _I, _I, _I, _P, _P, _P, _I, _P, _P, _S, _I, _P]),
     "kl_linear_workspace_bytes": (_S, [_I, _I, _I, _I, _I, _I]),
@@ -68,6 +74,11 @@ _SIGNATURES = {
     "kl_rmsnorm": (_I, [_P, _P, _P, _I, _I, _I, ctypes.c_float, _I, _P, _P, _P]),
     "kl_linear_topk": (_I, [_P, _I, _I, _I, _P, _I, _I, _I, _P, _P, _I, ctypes.c_longlong, _P, _P, _P, _S, _I, _P]),
     "kl_linear_topk_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
+    "kl_qk_norm_rope_write": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P,
+                                   ctypes.c_float, _P, _P, _P]),
+    "kl_read_kv": (_I, [_P, _I, _P, _I, _P, _P, _P]),
+    "kl_paged_attention": (_I, [_P, _L, _L, _I, _I, _I, _P, _P, _L, _I, _P, ctypes.c_float, _P, _P, _P, _S, _P]),
+    "kl_paged_attention_workspace_bytes": (_S, [_I, _I, _I, _I]),
 }
 
 _lib = None

@@ -883,6 +883,105 @@ int kl_rmsnorm(const void* x, const void* residual, const void* weight, int dtyp
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "rmsnorm launch");
 }
 
+namespace {
+
+int check_device(kl::DeviceInfo* di) {
+  const int rc = kl::device_info(di);
+  if (rc != KL_OK) return rc;
+  if (!(di->major == 10 && di->minor == 0))
+    return kl::fail(KL_ERR_UNSUPPORTED, "this library is built for sm_100a (device is sm%d%d)", di->major, di->minor);
+  return KL_OK;
+}
+
+// Checks of the cache that its three operators share; dtype is the activations'.
+int validate_cache(const kl_kv_cache* c, int dtype) {
+  if (!c || !c->k || !c->v) return fail(KL_ERR_INVALID, "the cache and its k and v must be non-null");
+  if (dtype != KL_DT_BF16 && dtype != KL_DT_F16) return fail(KL_ERR_INVALID, "the KV operators take bf16 or f16 (dtype %d)", dtype);
+  if (c->format != KL_KV_SAME && c->format != KL_KV_INT8) return fail(KL_ERR_INVALID, "unknown cache format %d", c->format);
+  if (c->format == KL_KV_INT8 && (!c->k_scales || !c->v_scales))
+    return fail(KL_ERR_INVALID, "an int8 cache needs k_scales and v_scales");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(KL_ERR_INVALID, "head_dim must be 64, 128 or 256 (%d)", c->head_dim);
+  if (c->pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0)
+    return fail(KL_ERR_INVALID, "need positive pages, page_size and kv_heads");
+  const long long unit = c->format == KL_KV_INT8 ? 16 : 8;
+  if (!aligned16(c->k) || !aligned16(c->v) || c->page_stride % unit || c->head_stride % unit || c->token_stride % unit)
+    return fail(KL_ERR_INVALID, "cache rows must be 16-byte aligned");
+  return KL_OK;
+}
+
+}  // namespace
+
+int kl_qk_norm_rope_write(const void* q, long long q_token_stride, long long q_head_stride, const void* k,
+                          long long k_token_stride, long long k_head_stride, const void* v, long long v_token_stride,
+                          long long v_head_stride, int dtype, int tokens, int heads, const void* q_weight,
+                          const void* k_weight, const float* cos, const float* sin, int max_positions,
+                          const int64_t* positions, const int64_t* slots, float eps, const kl_kv_cache* cache, void* q_out,
+                          void* stream) {
+  int rc = validate_cache(cache, dtype);
+  if (rc != KL_OK) return rc;
+  if (tokens < 0 || heads <= 0) return fail(KL_ERR_INVALID, "need tokens >= 0 and heads > 0");
+  if ((q_weight == nullptr) != (k_weight == nullptr))
+    return fail(KL_ERR_INVALID, "q_weight and k_weight must be given together");
+  if (q_weight && (!(eps > 0.0f) || !(eps < 3.0e38f))) return fail(KL_ERR_INVALID, "epsilon must be finite and positive");
+  if (max_positions <= 0) return fail(KL_ERR_INVALID, "the rotary table is empty");
+  if (tokens == 0) return KL_OK;
+  if (!q || !k || !v || !cos || !sin || !positions || !slots || !q_out)
+    return fail(KL_ERR_INVALID, "q, k, v, cos, sin, positions, slots and q_out must be non-null");
+  if (static_cast<long long>(tokens) * (heads + 2ll * cache->kv_heads) > 0x7FFFFFFFll)
+    return fail(KL_ERR_INVALID, "tokens * (heads + 2 kv_heads) must stay below 2^31");
+  DeviceInfo di;
+  if ((rc = check_device(&di)) != KL_OK) return rc;
+  const KvRows x[3] = {{q, q_token_stride, q_head_stride}, {k, k_token_stride, k_head_stride}, {v, v_token_stride, v_head_stride}};
+  const cudaError_t e = launch_kv_write(x, dtype, tokens, heads, q_weight, k_weight, cos, sin, max_positions, positions, slots,
+                                        eps, *cache, q_out, di.status, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "KV write launch");
+}
+
+int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int tokens, void* k, void* v, void* stream) {
+  int rc = validate_cache(cache, dtype);
+  if (rc != KL_OK) return rc;
+  if (tokens < 0) return fail(KL_ERR_INVALID, "need tokens >= 0");
+  if (tokens == 0) return KL_OK;
+  if (!slots || !k || !v) return fail(KL_ERR_INVALID, "slots, k and v must be non-null");
+  if (!aligned16(k) || !aligned16(v)) return fail(KL_ERR_INVALID, "k and v must be 16-byte aligned");
+  if (2ll * tokens * cache->kv_heads > 0x7FFFFFFFll) return fail(KL_ERR_INVALID, "2 * tokens * kv_heads must stay below 2^31");
+  DeviceInfo di;
+  if ((rc = check_device(&di)) != KL_OK) return rc;
+  const cudaError_t e = launch_kv_read(*cache, dtype, slots, tokens, k, v, di.status, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "KV read launch");
+}
+
+size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  return paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim, sm_count_or_default());
+}
+
+int kl_paged_attention(const void* q, long long q_row_stride, long long q_head_stride, int dtype, int batch, int heads,
+                       const kl_kv_cache* cache, const int32_t* page_table, long long table_stride, int columns,
+                       const int32_t* lengths, float scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  int rc = validate_cache(cache, dtype);
+  if (rc != KL_OK) return rc;
+  if (batch < 0 || heads <= 0 || columns < 0 || heads % cache->kv_heads)
+    return fail(KL_ERR_INVALID, "need batch >= 0, columns >= 0 and heads a multiple of kv_heads");
+  if (!(scale > -3.0e38f && scale < 3.0e38f)) return fail(KL_ERR_INVALID, "scale must be finite");
+  if (batch == 0) return KL_OK;
+  if (!q || !lengths || !out || (columns > 0 && !page_table)) return fail(KL_ERR_INVALID, "q, page_table, lengths and out must be non-null");
+  if (!aligned16(out)) return fail(KL_ERR_INVALID, "out must be 16-byte aligned");
+  if (static_cast<long long>(columns) * cache->page_size > 0x7FFFFFFFll || static_cast<long long>(batch) * heads > 0x7FFFFFFFll)
+    return fail(KL_ERR_INVALID, "columns * page_size and batch * heads must stay below 2^31");
+  DeviceInfo di;
+  if ((rc = check_device(&di)) != KL_OK) return rc;
+  const size_t need = paged_attention_workspace_bytes(batch, heads, cache->kv_heads, cache->head_dim, di.sm_count);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(KL_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : 0);
+  const cudaError_t e = launch_paged_attention(q, dtype, batch, heads, q_row_stride, q_head_stride, *cache, page_table, table_stride,
+                                               columns, lengths, scale, out, lse, workspace, di.sm_count, di.status,
+                                               static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? KL_OK : cuda_fail(e, "paged attention launch");
+}
+
 int kl_quantize_w8_row(const void* w, int w_dtype, int n, int k, int8_t* q, void* scale_bf16, void* stream) {
   if (!w || !q || !scale_bf16) return fail(KL_ERR_INVALID, "null pointer");
   if (n <= 0 || k <= 0) return fail(KL_ERR_INVALID, "weight must be a nonempty [N,K] matrix");

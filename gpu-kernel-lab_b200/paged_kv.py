@@ -1,0 +1,243 @@
+"""The paged key-value cache of a decoder layer: write, read back, attend.
+
+These are the steps between the quantized QKV projection and ``o_proj``:
+
+* ``qk_norm_rope_write``: RMSNorm of every query and key head, rotary positions
+  and the cache write, one launch for any number of tokens (the reference's
+  ``learning/08_decode/fused_qkv_cache.py:7-54``, on pages);
+* ``paged_attention``: attention of one new token per sequence over its pages
+  (``serving/paged_attention.py:11-101``);
+* ``read_kv``: cached keys and values of given slots, dequantised, for a
+  prompt's attention over a cached prefix (``serving/paged_gather.py:8-28``).
+
+A cache is ``k_cache`` and ``v_cache``, ``[pages, kv_heads, page_size,
+head_dim]`` with contiguous heads' elements and otherwise any (equal) strides:
+a cache laid out ``[pages, page_size, kv_heads, head_dim]`` is passed as
+``cache.transpose(1, 2)``.  It holds the activations' type (bf16 or f16), or int8
+codes with one f32 scale per token and head in ``k_scales`` and ``v_scales``
+``[pages, kv_heads, page_size]``.  ``new_kv_cache`` allocates one; ``kv_slots``
+turns positions into slots (``page * page_size + offset``).
+
+Arguments are checked on the host (``ValueError``).  What only the device sees
+(a position, slot, page id or length out of range) never leads to an access
+outside the buffers and is recorded for ``_native.device_status``.
+
+The functions are for inference: tensors that require grad are refused, as
+``qwen_rmsnorm`` refuses them.
+"""
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native as N
+
+HEAD_DIMS = (64, 128, 256)
+_CODES = {torch.bfloat16: N.KL_DT_BF16, torch.float16: N.KL_DT_F16}
+
+
+class KVCache(NamedTuple):
+    """``k_cache`` and ``v_cache``, and their scales where they are int8."""
+    k_cache: torch.Tensor
+    v_cache: torch.Tensor
+    k_scales: Optional[torch.Tensor] = None
+    v_scales: Optional[torch.Tensor] = None
+
+
+def new_kv_cache(pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda") -> KVCache:
+    """An empty cache; ``dtype`` is bf16, f16 or ``torch.int8``."""
+    if dtype not in (*_CODES, torch.int8):
+        raise ValueError('a cache holds bf16, f16 or int8')
+    if head_dim not in HEAD_DIMS:
+        raise ValueError('head_dim must be 64, 128 or 256')
+    if min(pages, page_size, kv_heads) < 1:
+        raise ValueError('pages, page_size and kv_heads must be positive')
+    k, v = (torch.zeros(pages, kv_heads, page_size, head_dim, dtype=dtype, device=device) for _ in range(2))
+    if dtype != torch.int8:
+        return KVCache(k, v)
+    return KVCache(k, v, *(torch.ones(pages, kv_heads, page_size, device=device) for _ in range(2)))
+
+
+def kv_slots(page_table, rows, positions, page_size):
+    """Slots (int64) of ``positions`` of the sequences ``rows`` of ``page_table``."""
+    return page_table[rows, positions // page_size].long() * page_size + positions % page_size
+
+
+def _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype):
+    """Checks of the cache that the three operators share, and its ``kl_kv_cache``."""
+    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError('k_cache and v_cache must be [pages, kv_heads, page_size, head_dim]')
+    pages, kv_heads, page_size, head_dim = k_cache.shape
+    strides = k_cache.stride()
+    if v_cache.stride() != strides or strides[3] != 1:
+        raise ValueError('k_cache and v_cache must have equal strides and contiguous head elements')
+    device = k_cache.device
+    if not k_cache.is_cuda or v_cache.device != device:
+        raise ValueError('the cache must be on one CUDA device')
+    if head_dim not in HEAD_DIMS:
+        raise ValueError('head_dim must be 64, 128 or 256')
+    if k_cache.dtype != v_cache.dtype:
+        raise ValueError('k_cache and v_cache must have one dtype')
+    if k_cache.dtype == torch.int8:
+        if k_scales is None or v_scales is None:
+            raise ValueError('an int8 cache needs k_scales and v_scales')
+        if k_scales.shape != k_cache.shape[:3] or v_scales.shape != k_cache.shape[:3] or k_scales.stride() != v_scales.stride():
+            raise ValueError('scales must be [pages, kv_heads, page_size] with equal strides')
+        if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.device != device or v_scales.device != device:
+            raise ValueError('scales must be FP32 on the cache\'s device')
+        return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), *strides[:3],
+                               *k_scales.stride(), N.KL_KV_INT8, pages, page_size, kv_heads, head_dim)
+    if k_scales is not None or v_scales is not None:
+        raise ValueError('only an int8 cache has scales')
+    if k_cache.dtype != dtype:
+        raise ValueError('the cache must be int8 or of the activations\' dtype')
+    return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, *strides[:3], 0, 0, 0, N.KL_KV_SAME, pages, page_size,
+                           kv_heads, head_dim)
+
+
+def _check_vector(t, name, dtype, count, device):
+    if t.shape != (count,) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+        raise ValueError(f'{name} must be a contiguous {dtype} vector of {count} on the cache\'s device')
+
+
+def _call(device, fn, *args):
+    """``fn(*args, stream)`` with ``device`` current."""
+    if device.index == torch.cuda.current_device():
+        N.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            N.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+
+
+def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales=None, v_scales=None,
+                       epsilon=1e-6):
+    """Normalise and rotate queries and keys, write keys and values to ``slots``; returns the queries.
+
+    * ``q`` ``[tokens, heads, head_dim]``, ``k`` and ``v`` ``[tokens, kv_heads, head_dim]``, bf16 or f16: any strides with
+      contiguous head elements, so views of a fused projection's output are taken as they are;
+    * ``q_weight``, ``k_weight`` ``[head_dim]``, or both None for a model without these norms;
+    * ``cos``, ``sin`` f32 ``[max_positions, head_dim / 2]``: element ``d`` rotates with ``d + head_dim / 2``;
+    * ``positions``, ``slots`` int64 ``[tokens]``; slots are distinct, a negative one is not cached.
+
+    The arithmetic is f32 up to one rounding at the store (an int8 cache quantises the f32 value).
+    """
+    if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError('q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]')
+    tokens, heads, dim = q.shape
+    dtype, device = q.dtype, q.device
+    if dtype not in _CODES or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError('q, k and v must have matching FP16/BF16 dtype')
+    if not q.is_cuda or k.device != device or v.device != device or k_cache.device != device:
+        raise ValueError('q, k, v and the cache must be on the same CUDA device')
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    if tokens and (sq[2] != 1 or sk[2] != 1 or sv[2] != 1):
+        raise ValueError('q, k and v must have contiguous head elements')
+    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype)
+    if k.shape[1] != k_cache.shape[1] or dim != k_cache.shape[3]:
+        raise ValueError('k and v must match the cache\'s heads and head_dim')
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError('q_weight and k_weight must be given together')
+    if q_weight is not None:
+        _check_vector(q_weight, 'q_weight', dtype, dim, device)
+        _check_vector(k_weight, 'k_weight', dtype, dim, device)
+        if not math.isfinite(epsilon) or epsilon <= 0:
+            raise ValueError('epsilon must be finite and positive')
+    if cos.ndim != 2 or cos.shape[0] == 0 or cos.shape[1] != dim // 2 or sin.shape != cos.shape:
+        raise ValueError('cos and sin must be [max_positions, head_dim / 2]')
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != device or sin.device != device
+            or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError('cos and sin must be contiguous FP32 on the cache\'s device')
+    _check_vector(positions, 'positions', torch.int64, tokens, device)
+    _check_vector(slots, 'slots', torch.int64, tokens, device)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise ValueError('inference only; use torch.inference_mode()')
+    out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+    if tokens:
+        _call(device, N.lib().kl_qk_norm_rope_write, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0],
+              sv[1], _CODES[dtype], tokens, heads, None if q_weight is None else q_weight.data_ptr(),
+              None if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+              positions.data_ptr(), slots.data_ptr(), epsilon, cache, out.data_ptr())
+    return out
+
+
+def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
+    """Keys and values ``[tokens, kv_heads, head_dim]`` of ``slots`` (int64), zeros for a negative slot.
+
+    ``dtype`` (bf16 or f16) is that of the result of an int8 cache, bf16 if not given; a 16-bit cache returns its own.
+    """
+    if dtype is None:
+        dtype = torch.bfloat16 if k_cache.dtype == torch.int8 else k_cache.dtype
+    if dtype not in _CODES:
+        raise ValueError('keys and values are read as FP16/BF16')
+    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype)
+    device, tokens = k_cache.device, slots.numel()
+    _check_vector(slots, 'slots', torch.int64, tokens, device)
+    shape = (tokens, k_cache.shape[1], k_cache.shape[3])
+    k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    if tokens:
+        _call(device, N.lib().kl_read_kv, cache, _CODES[dtype], slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None, return_lse=False,
+                    workspace=None):
+    """Attention of one new token per sequence: ``softmax(scale * q K^T) V`` over each sequence's cached tokens.
+
+    * ``q`` ``[batch, heads, head_dim]``, bf16 or f16, contiguous head elements; ``heads`` a multiple of the cache's;
+    * ``page_table`` int32 ``[batch, columns]``: page ``i`` of a sequence holds its tokens ``i * page_size ...``; entries
+      past its length are not read;
+    * ``lengths`` int32 ``[batch]``, the new token (written before) included; a sequence of length 0 gives zeros;
+    * ``scale`` is ``head_dim ** -0.5`` if not given.
+
+    Returns the output, or ``(output, lse)`` with ``return_lse``: f32 ``[batch, heads]``, the log of the sum of the
+    exponentials (``-inf`` for a length of 0), by which parts of a sequence can be joined.  ``workspace`` (uint8, zeroed
+    once, of ``paged_attention_workspace_bytes``) takes the place of the scratch kept per device and stream.
+    """
+    if q.ndim != 3:
+        raise ValueError('q must be [batch, heads, head_dim]')
+    batch, heads, dim = q.shape
+    dtype, device = q.dtype, q.device
+    if dtype not in _CODES:
+        raise ValueError('q must be FP16/BF16')
+    if not q.is_cuda or k_cache.device != device:
+        raise ValueError('q and the cache must be on the same CUDA device')
+    strides = q.stride()
+    if batch and strides[2] != 1:
+        raise ValueError('q must have contiguous head elements')
+    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype)
+    kv_heads = k_cache.shape[1]
+    if dim != k_cache.shape[3] or heads == 0 or heads % kv_heads:
+        raise ValueError('q must match the cache\'s head_dim and have a multiple of its heads')
+    if page_table.ndim != 2 or page_table.shape[0] != batch or page_table.dtype != torch.int32 or page_table.device != device:
+        raise ValueError('page_table must be int32 [batch, columns] on the cache\'s device')
+    table_stride, step = page_table.stride()
+    columns = page_table.shape[1]
+    if columns > 1 and step != 1:
+        raise ValueError('page_table must have contiguous rows')
+    _check_vector(lengths, 'lengths', torch.int32, batch, device)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError('scale must be finite')
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise ValueError('inference only; use torch.inference_mode()')
+    out = torch.empty((batch, heads, dim), dtype=dtype, device=device)
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+    if batch:
+        lib = N.lib()
+        if workspace is None:
+            need = lib.kl_paged_attention_workspace_bytes(batch, heads, kv_heads, dim)
+            workspace = N.workspace(device, need, stream=torch.cuda.current_stream(device))
+        elif workspace.device != device or not workspace.is_contiguous():
+            raise ValueError('workspace must be contiguous, on the cache\'s device')
+        _call(device, lib.kl_paged_attention, q.data_ptr(), strides[0], strides[1], _CODES[dtype], batch, heads, cache,
+              page_table.data_ptr(), table_stride, columns, lengths.data_ptr(), scale, out.data_ptr(),
+              None if lse is None else lse.data_ptr(), None if workspace is None else workspace.data_ptr(),
+              0 if workspace is None else workspace.numel() * workspace.element_size())
+    return (out, lse) if return_lse else out
+
+
+def paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim) -> int:
+    """Bytes of scratch that ``paged_attention`` needs, for a ``workspace`` of the caller's own."""
+    return N.lib().kl_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim)

@@ -286,6 +286,90 @@ int kl_rmsnorm(const void* x, const void* residual, const void* weight, int dtyp
                void* stream);
 
 /*
+ * Paged key-value cache: what stands between the QKV projection and o_proj of
+ * a decoder layer.  Keys and values of one token and KV head are head_dim
+ * contiguous elements; all strides are in elements and 64-bit.  K and V have
+ * the same shape and strides.  A slot is page * page_size + offset in the page.
+ *   KL_KV_SAME  the cache holds the activations' 16-bit type
+ *   KL_KV_INT8  int8 codes and one f32 scale per (page, head, token):
+ *               value = code * scale, scale = max|x| / 127 (1 for zeros),
+ *               code = rint(x / scale); a row with a NaN or an infinity gets a
+ *               NaN scale
+ * head_dim is 64, 128 or 256.  Bases are 16-byte aligned and the K/V strides
+ * multiples of 16 bytes.
+ */
+#define KL_KV_SAME 0
+#define KL_KV_INT8 1
+typedef struct kl_kv_cache {
+  void* k;                     /* [pages, kv_heads, page_size, head_dim] by the strides below */
+  void* v;
+  float* k_scales;             /* [pages, kv_heads, page_size]; KL_KV_INT8 only, else NULL    */
+  float* v_scales;
+  long long page_stride, head_stride, token_stride;
+  long long scale_page_stride, scale_head_stride, scale_token_stride;
+  int format, pages, page_size, kv_heads, head_dim;
+} kl_kv_cache;
+
+/*
+ * RMSNorm of every query and key head, rotary positions, and the write of keys
+ * and values into the cache, in one pass (the work of the reference's
+ * learning/08_decode/fused_qkv_cache.py:7-54 on a paged cache, for any number
+ * of tokens).
+ *   y  = x * rsqrt(mean(x^2) + eps) * weight          (weights NULL: y = x)
+ *   y' = (y_a * c - y_b * s, y_b * c + y_a * s)       halves a and b of the head
+ * in f32, rounded once.  The values are written unchanged (or quantised).
+ *   q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]: dtype
+ *   bf16 or f16, elements contiguous, strides in elements (views of a fused
+ *   QKV projection's output need no copy).
+ *   q_weight, k_weight [head_dim] of the same type, both or neither.
+ *   cos, sin f32 [max_positions, head_dim / 2]; positions, slots int64 [tokens].
+ *   A negative slot is not cached (its query is still written); slots are
+ *   otherwise distinct.  A position or slot out of range records
+ *   KL_ERR_INVALID in the device status word; such a slot is not written and
+ *   such a position is taken as 0.
+ *   q_out [tokens, heads, head_dim] contiguous; it may be q only where q is
+ *   contiguous too.
+ */
+int kl_qk_norm_rope_write(const void* q, long long q_token_stride, long long q_head_stride,
+                          const void* k, long long k_token_stride, long long k_head_stride,
+                          const void* v, long long v_token_stride, long long v_head_stride,
+                          int dtype, int tokens, int heads, const void* q_weight, const void* k_weight,
+                          const float* cos, const float* sin, int max_positions, const int64_t* positions,
+                          const int64_t* slots, float eps, const kl_kv_cache* cache, void* q_out, void* stream);
+
+/*
+ * Keys and values of the given slots, dequantised: k and v [tokens, kv_heads,
+ * head_dim] contiguous in dtype (the cache's own type for KL_KV_SAME).  The role
+ * of the reference's serving/paged_gather.py:8-28.  A negative slot
+ * gives zeros; a slot out of range gives zeros and records KL_ERR_INVALID in
+ * the device status word.
+ */
+int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int tokens, void* k, void* v, void* stream);
+
+/*
+ * Attention of one new token per sequence over the paged cache (the role of
+ * the reference's serving/paged_attention.py:11-101):
+ *   out[b, h] = softmax_j(scale * q[b, h] . K[j]) V,   j < lengths[b]
+ * where key j of sequence b is in page page_table[b, j / page_size] and query
+ * head h reads KV head h / (heads / kv_heads).
+ *   q [batch, heads, head_dim] bf16 or f16, elements contiguous; out
+ *   [batch, heads, head_dim] contiguous; lse f32 [batch, heads] or NULL: the
+ *   natural log of the sum of exp(scores).  lengths[b] <= 0: zeros, lse -inf.
+ *   page_table int32 [batch, columns] by table_stride (elements).  Its entries
+ *   past a sequence's length are not read.  A length beyond columns *
+ *   page_size is cut to it, and keys of a page id out of range count
+ *   as absent; both record KL_ERR_INVALID in the device status word.
+ *   workspace: kl_paged_attention_workspace_bytes(...) bytes under kl_linear's
+ *   workspace rule (its first 64 KiB zero before the first use; the calls leave
+ *   it zero).
+ */
+size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim);
+int kl_paged_attention(const void* q, long long q_row_stride, long long q_head_stride, int dtype, int batch, int heads,
+                       const kl_kv_cache* cache, const int32_t* page_table, long long table_stride, int columns,
+                       const int32_t* lengths, float scale, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Host-only description of the launch plan kl_linear would use on a device
  * with `sm_count` SMs, and a self-check of its work partition (every
  * (tile, k-block) unit covered exactly once, workspace slots in bounds).
