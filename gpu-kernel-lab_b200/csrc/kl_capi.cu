@@ -969,13 +969,14 @@ int kl_paged_attention(const void* q, long long q_row_stride, long long q_head_s
   if (batch == 0) return KL_OK;
   if (!q || !lengths || !out || (columns > 0 && !page_table)) return fail(KL_ERR_INVALID, "q, page_table, lengths and out must be non-null");
   if (!aligned16(out)) return fail(KL_ERR_INVALID, "out must be 16-byte aligned");
-  if (static_cast<long long>(columns) * cache->page_size > 0x7FFFFFFFll || static_cast<long long>(batch) * heads > 0x7FFFFFFFll)
+  if (static_cast<long long>(columns) * cache->page_size > 0x7FFF0000ll || static_cast<long long>(batch) * heads > 0x7FFFFFFFll)
     return fail(KL_ERR_INVALID, "columns * page_size and batch * heads must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
   const size_t need = paged_attention_workspace_bytes(batch, heads, cache->kv_heads, cache->head_dim, di.sm_count);
   if (need && (!workspace || workspace_bytes < need))
     return fail(KL_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : 0);
+  if (!aligned16(workspace)) return fail(KL_ERR_INVALID, "workspace must be 16-byte aligned");
   const cudaError_t e = launch_paged_attention(q, dtype, batch, heads, q_row_stride, q_head_stride, *cache, page_table, table_stride,
                                                columns, lengths, scale, out, lse, workspace, di.sm_count, di.status,
                                                static_cast<cudaStream_t>(stream));
