@@ -934,7 +934,7 @@ int kl_qk_norm_rope_write(const void* q, long long q_token_stride, long long q_h
   if ((rc = check_device(&di)) != KL_OK) return rc;
   const KvRows x[3] = {{q, q_token_stride, q_head_stride}, {k, k_token_stride, k_head_stride}, {v, v_token_stride, v_head_stride}};
   const cudaError_t e = launch_kv_write(x, dtype, tokens, heads, q_weight, k_weight, cos, sin, max_positions, positions, slots,
-                                        eps, *cache, q_out, di.status, static_cast<cudaStream_t>(stream));
+                                        eps, *cache, q_out, di.sm_count, di.status, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "KV write launch");
 }
 
@@ -944,11 +944,12 @@ int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int to
   if (tokens < 0) return fail(KL_ERR_INVALID, "need tokens >= 0");
   if (tokens == 0) return KL_OK;
   if (!slots || !k || !v) return fail(KL_ERR_INVALID, "slots, k and v must be non-null");
-  if (!aligned16(k) || !aligned16(v)) return fail(KL_ERR_INVALID, "k and v must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31u)
+    return fail(KL_ERR_INVALID, "k and v must be 32-byte aligned");
   if (2ll * tokens * cache->kv_heads > 0x7FFFFFFFll) return fail(KL_ERR_INVALID, "2 * tokens * kv_heads must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
-  const cudaError_t e = launch_kv_read(*cache, dtype, slots, tokens, k, v, di.status, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_kv_read(*cache, dtype, slots, tokens, k, v, di.sm_count, di.status, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "KV read launch");
 }
 

@@ -255,10 +255,10 @@ struct KvRows {
 // x: the rows of q, k and v; q_weight/k_weight both null without the norm (kl_kv.cu)
 cudaError_t launch_kv_write(const KvRows x[3], int dtype, int tokens, int heads, const void* q_weight, const void* k_weight,
                             const float* cos, const float* sin, int max_positions, const int64_t* positions,
-                            const int64_t* slots, float eps, const kl_kv_cache& cache, void* q_out, int* status,
-                            cudaStream_t s);
-cudaError_t launch_kv_read(const kl_kv_cache& cache, int dtype, const int64_t* slots, int tokens, void* k, void* v, int* status,
-                           cudaStream_t s);
+                            const int64_t* slots, float eps, const kl_kv_cache& cache, void* q_out, int sm_count,
+                            int* status, cudaStream_t s);
+cudaError_t launch_kv_read(const kl_kv_cache& cache, int dtype, const int64_t* slots, int tokens, void* k, void* v,
+                           int sm_count, int* status, cudaStream_t s);
 // kl_paged_attention.cu
 size_t paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int sm_count);
 cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int heads, long long q_row_stride,

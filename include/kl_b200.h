@@ -339,7 +339,8 @@ int kl_qk_norm_rope_write(const void* q, long long q_token_stride, long long q_h
 
 /*
  * Keys and values of the given slots, dequantised: k and v [tokens, kv_heads,
- * head_dim] contiguous in dtype (the cache's own type for KL_KV_SAME).  The role
+ * head_dim] contiguous in dtype (the cache's own type for KL_KV_SAME), 32-byte
+ * aligned.  The role
  * of the reference's serving/paged_gather.py:8-28.  A negative slot
  * gives zeros; a slot out of range gives zeros and records KL_ERR_INVALID in
  * the device status word.
