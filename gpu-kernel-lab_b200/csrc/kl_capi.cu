@@ -199,6 +199,8 @@ int report_error(int code, const char* fmt, ...) {
   return code;
 }
 
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
+
 }  // namespace kl
 
 using namespace kl;

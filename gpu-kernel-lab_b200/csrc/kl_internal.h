@@ -259,6 +259,8 @@ cudaError_t launch_kv_write(const KvRows x[3], int dtype, int tokens, int heads,
                             int* status, cudaStream_t s);
 cudaError_t launch_kv_read(const kl_kv_cache& cache, int dtype, const int64_t* slots, int tokens, void* k, void* v,
                            int sm_count, int* status, cudaStream_t s);
+// cuTensorMapEncodeTiled (PFN_cuTensorMapEncodeTiled_v12000), or null
+void* tensor_map_encoder();
 // kl_paged_attention.cu
 size_t paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int sm_count);
 cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int heads, long long q_row_stride,

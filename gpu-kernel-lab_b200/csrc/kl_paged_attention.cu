@@ -26,11 +26,13 @@
 // second product as two 16-bit numbers p = hi + lo (16 bits of bf16 or 22 of
 // f16), so that their rounding stays below the output's. With up to four heads per KV
 // head the heads stand twice in the eight columns and the second copy carries
-// lo: no instruction more. Int8 keys become f16 (exact) against queries scaled by a
-// power of two into f16's range (a bf16 query loses nothing down to 2^-28 of its
-// head's largest); the key's scale multiplies the score. Int8 values become
-// bf16 (exact), their scale multiplies the weight.
+// lo: no instruction more. Int8 keys and values are
+// converted exactly (to q / 64 in bf16, where the products are in bf16); the key's
+// scale multiplies the score, the value's scale the weight.
+#include <atomic>
 #include <cfloat>
+
+#include <cudaTypedefs.h>
 
 #include "kl_internal.h"
 #include "kl_kv.cuh"
@@ -40,8 +42,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr int kMaxLens = 512;          // lengths kept in shared memory
+constexpr float kSlack = 8.0f;           // log2 of how far weights may exceed 1
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -55,7 +58,10 @@ struct AttnArgs {
   int batch, heads, columns;
   int group;                           // query heads per KV head
   int blocks;                          // blocks of HB query heads per KV head
-  int q_vec;                           // q rows allow 8-byte loads
+  int q_vec;                           // q rows allow 4-byte loads
+  int box;                             // rows of one TMA box (divides the page), 0: copies by the lanes
+  uint32_t page_mul;                   // position / page_size = position * page_mul >> page_shift
+  int page_shift;
   float scale;
   void* out;
   float* lse;
@@ -63,6 +69,25 @@ struct AttnArgs {
   float* partials;
   int* status;
 };
+
+struct alignas(64) AttnMaps {
+  CUtensorMap k, v;                    // [page, head, token, element]
+  CUtensorMap ks, vs;                  // [page, head, token], int8 only
+};
+
+KL_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
+KL_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
+// One of the barrier's arrivals, once this thread's earlier cp.async copies have landed
+KL_DEVICE void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
+}
 
 KL_DEVICE float ex2(float x) {
   float y;
@@ -108,10 +133,15 @@ template <bool BF16> KL_DEVICE float2 unpack2(uint32_t v) {
 template <uint32_t SEL> KL_DEVICE uint32_t s8_to_f16(uint32_t w) {
   return fma_f16x2(prmt(w, 0x64646464u, SEL), 0x3C003C00u, 0xE480E480u);
 }
-// Two int8 values, bytes SEL of w, to exact bf16: 0x4300 | low 7 bits is 128 + v, 0x4300 | sign bit is 128 or 256.
-template <uint32_t SEL> KL_DEVICE uint32_t s8_to_bf16(uint32_t w) {
-  const uint32_t t = prmt(w, 0x43434343u, SEL);
-  return fma_bf16x2((t & 0x00800080u) | 0x43004300u, 0xBF80BF80u, t & 0xFF7FFF7Fu);
+// Two int8 values, bytes SEL of w, to exact bf16 q / 64: the bits 0x00uu of u = q ^ 0x80 are
+// u * 2^-133 (subnormals and the first binade have one step), and 2^127 u * 2^-133 - 2 = (u - 128) / 64.
+template <uint32_t SEL> KL_DEVICE uint32_t s8_to_bf16_64th(uint32_t w) {
+  return fma_bf16x2(prmt(w, 0, SEL), 0x7F007F00u, 0xC000C000u);
+}
+// ... of keys, in the type of the queries
+template <bool BF16, uint32_t SEL> KL_DEVICE uint32_t s8_to_key(uint32_t w) {
+  if constexpr (BF16) return s8_to_bf16_64th<SEL>(w);
+  else return s8_to_f16<SEL>(w);
 }
 
 KL_DEVICE uint32_t load16(const void* p) { return *static_cast<const unsigned short*>(p); }
@@ -132,34 +162,40 @@ struct Geo {
   static constexpr int kNT = HB == 16 ? 2 : 1;                    // column tiles
   static constexpr bool kDup = HB == 4;
   static constexpr int kCols = 8 * kNT;
-  static constexpr int kKV = 2 * kKeys * kRow;
-  static constexpr int kOutRow = D + 4;                           // floats; the pad spreads columns over the banks
-  static constexpr int kOut = kCols * kOutRow * 4;                // a warp's output, over its consumed slot
-  static constexpr int kScales = INT8 ? 2 * kKeys * 4 : 0;
-  static constexpr int kSlotRaw = kKV + kScales + 16;             // + the mask of the valid keys
-  static constexpr int kSlot = ((kSlotRaw > kOut ? kSlotRaw : kOut) + 127) / 128 * 128;
-  static constexpr int kRing = kWarps * kStages * kSlot;
+  static constexpr int kKV = 2 * kKeys * kRow;                    // one slot of a warp's ring
+  static constexpr int kSpan = kRow < 128 ? kRow : 128;           // bytes of a key in one swizzled segment
+  static constexpr int kSegs = kRow / kSpan;
+  static constexpr int kRing = kWarps * kStages * kKV;
+  static constexpr int kScales = kTiles * 128;                    // bytes for a slot's key (or value) scales
+  static constexpr int kNote = (INT8 ? 2 * kScales : 0) + 128;    // per slot: the scales, and the mask of the valid keys
   static constexpr int kStats = 2 * kWarps * kCols * 4;           // every warp's maximum and sum per column
-  static constexpr int kSmem = kRing + kStats + kMaxLens * 4 + 128;
+  static constexpr int kSmem = 1024 + kRing + kWarps * kStages * (kNote + 8) + kStats + kMaxLens * 4 + 64;
+  static constexpr int kResident = kSmem > 113 * 1024 ? 1 : HB == 16 || D == 256 ? 2 : 3;   // CTAs per SM
+  static_assert(kCols * D * 4 <= kKV, "a warp's output goes over its consumed slot");
   static constexpr int kPartial = HB * (D + 2);                   // floats of one partial row
-  static_assert(kKeys <= 64, "");
+  static_assert(kKeys <= 64 && kNote % 128 == 0, "");
 };
 
 struct Cursor {
-  int b, r, i;         // sequence, row of the sequence, unit of the row
+  int b, head, block, i;   // sequence, KV head, block of its query heads, unit of that row
   int units, len;
 };
 
 template <typename T, bool INT8, int D, int HB>
-__global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 1024 ? 2 : 1) attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
+    attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps) {
   using G = Geo<INT8, D, HB>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr bool kQkBf16 = kBf16 && !INT8;          // type of the K Q^T product
+  constexpr bool kQkBf16 = kBf16;                   // type of the K Q^T product
   constexpr bool kPvBf16 = kBf16 || INT8;           // type of the V^T P^T product
   constexpr int kChunks = G::kRow / 16;             // 16-byte chunks of one key
   constexpr int kRowsPer = 32 / kChunks;            // keys that one warp-wide copy covers
-  extern __shared__ __align__(128) char smem[];
-  float* s_max = reinterpret_cast<float*>(smem + G::kRing);
+  constexpr int kWords = (G::kKeys + 31) / 32;      // keys per lane
+  extern __shared__ char smem_raw[];
+  char* const smem = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
+  char* const notes = smem + G::kRing;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(notes + kWarps * kStages * G::kNote);
+  float* s_max = reinterpret_cast<float*>(bars + kWarps * kStages);
   float* s_sum = s_max + kWarps * G::kCols;
   int* s_len = reinterpret_cast<int*>(s_sum + kWarps * G::kCols);
   int* s_misc = s_len + kMaxLens;                   // [0..7] scan totals, [8] start b, [9] start rest, [10] last flag
@@ -192,6 +228,8 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
   }
   long long* s_tot = reinterpret_cast<long long*>(s_misc);
   if (lane == 31) s_tot[warp] = incl;
+  if (tid < kWarps * kStages) mbar_init(smem_u32(bars + tid), a.box ? 1 : 33);
+  if (tid == 0) fence_mbar_init();
   __syncthreads();
   long long total = 0;
 #pragma unroll
@@ -230,8 +268,10 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
   auto advance = [&](Cursor& c) {
     if (++c.i < c.units) return;
     c.i = 0;
-    if (++c.r < rows) return;
-    c.r = 0;
+    if (++c.block < a.blocks) return;
+    c.block = 0;
+    if (++c.head < a.kv.kv_heads) return;
+    c.head = 0;
     do {
       if (++c.b >= a.batch) return;
       load_len(c);
@@ -240,79 +280,124 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
   Cursor in;                                        // next unit to fetch
   in.b = s_misc[8];
   load_len(in);
-  in.r = s_misc[9] / in.units;
   in.i = s_misc[9] % in.units;
+  in.head = s_misc[9] / in.units / a.blocks;
+  in.block = s_misc[9] / in.units % a.blocks;
   Cursor at = in;                                   // unit being computed
 
   // ---- fetching: this warp's keys of the unit `in` into ring slot `slot`
-  const uint32_t ring = smem_u32(smem) + warp * kStages * G::kSlot;
-  char* const ring_ptr = smem + warp * kStages * G::kSlot;
-  const int chunk = lane % kChunks, row0 = lane / kChunks;
-  const long long delta = a.kv.v - a.kv.k;
-  auto fetch = [&](int slot) {
-    const uint32_t dst = ring + slot * G::kSlot;
-    const int pos0 = in.i * G::kUnit + warp * G::kKeys;
-    const int count = min(G::kKeys, in.len - pos0);             // may be <= 0
-    const int head = in.r / a.blocks;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * G::kKV;
+  char* const ring_ptr = smem + warp * kStages * G::kKV;
+  char* const note = notes + warp * kStages * G::kNote;
+  const uint32_t bar = smem_u32(bars + warp * kStages);
+  auto place = [&](uint32_t base, int row, int c) {          // chunk c of key `row` in a slot's K or V part
+    if constexpr (G::kSpan == 64) return base + row * 64 + (c ^ ((row >> 1) & 3)) * 16;
+    else return base + (c >> 3) * (G::kKeys * 128) + row * 128 + ((c & 7) ^ (row & 7)) * 16;
+  };
+  int page[kWords];                                 // of the lane's keys, and their place in it: read a unit ahead
+  unsigned rest[kWords];
+  auto look_up = [&]() {
     const int* table = a.table + in.b * a.table_stride;
-    unsigned valid[(G::kKeys + 31) / 32];
+    const int pos0 = in.i * G::kUnit + warp * G::kKeys;
 #pragma unroll
-    for (int w = 0; w < (G::kKeys + 31) / 32; ++w) valid[w] = 0;
-    // lane's row offset in the cache (elements), and its scale's; one or two rows per lane
-    long long off[(G::kKeys + 31) / 32], soff[(G::kKeys + 31) / 32];
-#pragma unroll
-    for (int w = 0; w < (G::kKeys + 31) / 32; ++w) {
-      const int row = w * 32 + lane;
-      bool ok = row < G::kKeys && row < count;
-      off[w] = soff[w] = 0;
-      if (ok) {
-        const unsigned pos = pos0 + row, column = pos / a.kv.page_size, rest = pos - column * a.kv.page_size;
-        const int page = table[column];
-        if (page < 0 || page >= a.kv.pages) {
-          record_error(a.status, KL_ERR_INVALID);
-          ok = false;
-        } else {
-          off[w] = page * a.kv.page_stride + head * a.kv.head_stride + rest * a.kv.token_stride;
-          if constexpr (INT8) soff[w] = page * a.kv.s_page_stride + head * a.kv.s_head_stride + rest * a.kv.s_token_stride;
-        }
-      }
-      valid[w] = __ballot_sync(0xFFFFFFFFu, ok);
-      if constexpr (INT8) {
-        if (row < G::kKeys) {
-          cp_async4(dst + G::kKV + row * 4, a.kv.ks + soff[w], ok ? 4 : 0);
-          cp_async4(dst + G::kKV + (G::kKeys + row) * 4, a.kv.vs + soff[w], ok ? 4 : 0);
-        }
-      }
+    for (int w = 0; w < kWords; ++w) {
+      const int row = w * 32 + lane, pos = pos0 + row;
+      const unsigned column = static_cast<unsigned>(static_cast<uint64_t>(static_cast<unsigned>(pos)) * a.page_mul >> a.page_shift);
+      rest[w] = pos - column * a.kv.page_size;
+      page[w] = row < G::kKeys && pos < in.len ? __ldg(table + column) : 0;
     }
-    if (lane == 0) {
-#pragma unroll
-      for (int w = 0; w < (G::kKeys + 31) / 32; ++w)
-        *reinterpret_cast<unsigned*>(ring_ptr + slot * G::kSlot + G::kKV + G::kScales + 4 * w) = valid[w];
-    }
+  };
+  uint32_t armed = 0, phases = 0;                   // per slot: copies under way, parity of its barrier
+  bool holey = false;
+  const int group_gap = a.box == 16 ? 32 : 16;      // floats from the scales of 16 keys to the next: a box starts at 128 bytes
+  auto fetch = [&](int slot) {
+    const int count = in.len - (in.i * G::kUnit + warp * G::kKeys);
     if (count <= 0) return;
+    armed |= 1u << slot;
+    const uint32_t dst = ring + slot * G::kKV, full = bar + slot * 8, scales = smem_u32(note) + slot * G::kNote;
+    bool used[kWords], bad = false;
 #pragma unroll
-    for (int j = 0; j < G::kKeys / kRowsPer; ++j) {
-      const int row = j * kRowsPer + row0;
-      const long long o = __shfl_sync(0xFFFFFFFFu, off[j * kRowsPer / 32], row & 31);
-      const int bytes = (valid[j * kRowsPer / 32] >> (row & 31)) & 1 ? 16 : 0;
-      const int swz = G::kRow == 64 ? chunk ^ ((row >> 1) & 3) : chunk ^ (row & 7);
-      const char* src = a.kv.k + o * G::kElem + chunk * 16;
-      const uint32_t d = dst + row * G::kRow + swz * 16;
-      cp_async16(d, src, bytes);
-      cp_async16(d + G::kKeys * G::kRow, src + delta, bytes);
+    for (int w = 0; w < kWords; ++w) {
+      const int row = w * 32 + lane;
+      used[w] = row < G::kKeys && row < count;
+      if (used[w] && static_cast<unsigned>(page[w]) >= static_cast<unsigned>(a.kv.pages)) used[w] = false, bad = true;
+    }
+    holey |= __any_sync(0xFFFFFFFFu, bad);
+    if (holey) {                                    // some page id was out of range: its keys count as absent
+      if (bad) record_error(a.status, KL_ERR_INVALID);
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        const unsigned v = __ballot_sync(0xFFFFFFFFu, used[w]);
+        if (lane == 0) reinterpret_cast<unsigned*>(note + slot * G::kNote + G::kNote - 128)[w] = v;
+      }
+    }
+    if (a.box) {
+      unsigned boxes = 0;
+      bool lead[kWords];
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        lead[w] = used[w] && (lane & (a.box - 1)) == 0 && (w == 0 || a.box < 64);
+        boxes += __popc(__ballot_sync(0xFFFFFFFFu, lead[w]));
+      }
+      if (lane == 0) mbar_arrive_expect_tx(full, boxes * a.box * (2 * G::kRow + (INT8 ? 8 : 0)));
+      __syncwarp();
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        if (lead[w]) {
+          const int row = w * 32 + lane;
+#pragma unroll
+          for (int g = 0; g < G::kSegs; ++g) {
+            const uint32_t to = dst + g * (G::kKeys * 128) + row * G::kSpan;
+            tma_load_4d(to, &maps.k, g * (G::kSpan / G::kElem), rest[w], in.head, page[w], full);
+            tma_load_4d(to + G::kKeys * G::kRow, &maps.v, g * (G::kSpan / G::kElem), rest[w], in.head, page[w], full);
+          }
+          if constexpr (INT8) {
+            tma_load_3d(scales + row / 4 * group_gap, &maps.ks, rest[w], in.head, page[w], full);
+            tma_load_3d(scales + G::kScales + row / 4 * group_gap, &maps.vs, rest[w], in.head, page[w], full);
+          }
+        }
+      }
+    } else {
+      const int chunk = lane % kChunks, row0 = lane / kChunks;
+      const long long delta = a.kv.v - a.kv.k;
+      long long off[kWords];
+      unsigned valid[kWords];
+#pragma unroll
+      for (int w = 0; w < kWords; ++w) {
+        off[w] = used[w] ? page[w] * a.kv.page_stride + in.head * a.kv.head_stride + rest[w] * a.kv.token_stride : 0;
+        valid[w] = __ballot_sync(0xFFFFFFFFu, used[w]);
+        if constexpr (INT8) {
+          const int row = w * 32 + lane;
+          if (row < G::kKeys) {
+            const long long from = used[w] ? page[w] * a.kv.s_page_stride + in.head * a.kv.s_head_stride + rest[w] * a.kv.s_token_stride : 0;
+            cp_async4(scales + row * 4, a.kv.ks + from, used[w] ? 4 : 0);
+            cp_async4(scales + G::kScales + row * 4, a.kv.vs + from, used[w] ? 4 : 0);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < G::kKeys / kRowsPer; ++j) {
+        const int row = j * kRowsPer + row0;
+        const long long o = __shfl_sync(0xFFFFFFFFu, off[j * kRowsPer / 32], row & 31);
+        const int bytes = (valid[j * kRowsPer / 32] >> (row & 31)) & 1 ? 16 : 0;
+        const char* src = a.kv.k + o * G::kElem + chunk * 16;
+        const uint32_t to = place(dst, row, chunk);
+        cp_async16(to, src, bytes);
+        cp_async16(to + G::kKeys * G::kRow, src + delta, bytes);
+      }
+      cp_async_arrive(full);
+      if (lane == 0) mbar_arrive(full);
     }
   };
 
   // ---- per-row state
   uint32_t qf[G::kNT][D / 16][2];
-  float qscale[G::kNT][2];                          // of the score columns 2 t4, 2 t4 + 1
+  const float qscale = a.scale * kLog2e * (INT8 && kBf16 ? 64.0f : 1.0f);
   float acc[D / 16][G::kNT][4];
   float top[G::kNT][2], sum[G::kNT][2];
   auto start_row = [&]() {
-    const int kvh = at.r / a.blocks, first = kvh * a.group + (at.r % a.blocks) * HB;
-    const int n = min(HB, (kvh + 1) * a.group - first);
+    const int first = at.head * a.group + at.block * HB, n = min(HB, a.group - at.block * HB);
     const char* q = static_cast<const char*>(a.q) + (at.b * a.q_row_stride + first * a.q_head_stride) * 2;
-    const float base = a.scale * kLog2e;
 #pragma unroll
     for (int nt = 0; nt < G::kNT; ++nt) {
       const int col = G::kDup ? (l4 & 3) : nt * 8 + l4;
@@ -324,34 +409,8 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
         qf[nt][ks][0] = there ? load_pair(p + d0 * 2, a.q_vec) : 0;
         qf[nt][ks][1] = there ? load_pair(p + d1 * 2, a.q_vec) : 0;
       }
-      float up = 1.0f;                              // bf16 against int8: the column's power of two
-      if constexpr (INT8 && kBf16) {
-        float big = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 f = unpack2<true>(qf[nt][ks][e]);
-            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-        // largest element into [2^14, 2^15); both factors stay normal numbers
-        int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
-        e = big == 0.0f || e == 128 ? 14 : max(e, -100);
-        const float down = __uint_as_float(static_cast<uint32_t>(14 - e + 127 > 254 ? 254 : 14 - e + 127) << 23);
-        up = 1.0f / down;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float2 f = unpack2<true>(qf[nt][ks][x]);
-            qf[nt][ks][x] = pack2<false>(f.x * down, f.y * down);
-          }
-      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        qscale[nt][e] = base * __shfl_sync(0xFFFFFFFFu, up, (2 * t4 + e) * 4);
         top[nt][e] = -FLT_MAX;                      // finite: a score of -inf has weight 0 and makes no NaN
         sum[nt][e] = 0.0f;
       }
@@ -364,17 +423,46 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
         for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
   };
 
-  auto swizzled = [&](uint32_t base, int row, int c) {
-    return base + row * G::kRow + (G::kRow == 64 ? c ^ ((row >> 1) & 3) : c ^ (row & 7)) * 16;
-  };
-
   // ---- one unit of this warp
+  bool dead = false;                                // a wait ran out: nothing more is fetched
   auto compute = [&](int slot) {
-    const uint32_t kbase = ring + slot * G::kSlot, vbase = kbase + G::kKeys * G::kRow;
-    const char* sp = ring_ptr + slot * G::kSlot + G::kKV;
-    const unsigned* mask = reinterpret_cast<const unsigned*>(sp + G::kScales);
-    const float* ksc = reinterpret_cast<const float*>(sp);
-    if (mask[0] == 0 && (G::kKeys <= 32 || mask[1] == 0)) return;
+    if (at.len <= at.i * G::kUnit + warp * G::kKeys) return;
+    const uint32_t kbase = ring + slot * G::kKV, vbase = kbase + G::kKeys * G::kRow;
+    const float* ksc = reinterpret_cast<const float*>(note + slot * G::kNote);
+    const float* vsc = ksc + G::kScales / 4;
+    if (armed >> slot & 1) {
+      if (!mbar_wait_time(bar + slot * 8, phases >> slot & 1)) {
+        dead = true;
+        record_error(a.status, KL_ERR_TIMEOUT);
+      }
+      armed ^= 1u << slot;
+      phases ^= 1u << slot;
+    }
+    __syncwarp();
+    const int count = at.len - (at.i * G::kUnit + warp * G::kKeys);
+    const bool partial = count < G::kKeys || holey;
+    unsigned valid[kWords];
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      valid[w] = count >= 32 * w + 32 ? 0xFFFFFFFFu : count <= 32 * w ? 0u : (1u << (count - 32 * w)) - 1;
+      if (holey) valid[w] &= reinterpret_cast<const unsigned*>(note + slot * G::kNote + G::kNote - 128)[w];
+    }
+    if (!INT8 && partial && a.box) {                // a box brings what the page holds past the length: values become 0
+      for (int i = lane; i < G::kKeys * G::kRow / 16; i += 32) {
+        const int row = i / (G::kSpan / 16) % G::kKeys;
+        if (!(valid[kWords == 1 ? 0 : row / 32] >> (row & 31) & 1))
+          *reinterpret_cast<uint4*>(ring_ptr + slot * G::kKV + G::kKeys * G::kRow + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    // chunk c of a row is at the row's chunk 0 or 1 with c * 16 exclusive-ored in (c even)
+    const uint32_t krow = place(kbase, (lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
+    const uint32_t vrow = INT8 ? place(vbase, (lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4)
+                               : place(vbase, (lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
+    auto cell = [](uint32_t row, int g, int c) {
+      return (row ^ ((c & (G::kSpan / 16 - 1)) * 16)) + (c / (G::kSpan / 16)) * (G::kKeys * G::kSpan) + g * 16 * G::kSpan;
+    };
     float s[G::kTiles][G::kNT][4];
 #pragma unroll
     for (int g = 0; g < G::kTiles; ++g) {
@@ -382,87 +470,118 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
       for (int nt = 0; nt < G::kNT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[g][nt][e] = 0.0f;
-      const int krow = g * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
       if constexpr (INT8) {
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
           uint32_t r[4];
-          ldsm4(r, swizzled(kbase, krow, c + (lane >> 4)));
+          ldsm4(r, cell(krow, g, c));
 #pragma unroll
           for (int x = 0; x < 4; ++x) r[x] ^= 0x80808080u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = s8_to_f16<0x4140>(r[2 * h]), a2 = s8_to_f16<0x4342>(r[2 * h]);
-            const uint32_t a1 = s8_to_f16<0x4140>(r[2 * h + 1]), a3 = s8_to_f16<0x4342>(r[2 * h + 1]);
+            const uint32_t a0 = s8_to_key<kBf16, 0x4140>(r[2 * h]), a2 = s8_to_key<kBf16, 0x4342>(r[2 * h]);
+            const uint32_t a1 = s8_to_key<kBf16, 0x4140>(r[2 * h + 1]), a3 = s8_to_key<kBf16, 0x4342>(r[2 * h + 1]);
 #pragma unroll
-            for (int nt = 0; nt < G::kNT; ++nt) mma16816<false>(s[g][nt], a0, a1, a2, a3, qf[nt][c + h][0], qf[nt][c + h][1]);
+            for (int nt = 0; nt < G::kNT; ++nt) mma16816<kQkBf16>(s[g][nt], a0, a1, a2, a3, qf[nt][c + h][0], qf[nt][c + h][1]);
           }
         }
       } else {
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           uint32_t r[4];
-          ldsm4(r, swizzled(kbase, krow, 2 * ks + (lane >> 4)));
+          ldsm4(r, cell(krow, g, 2 * ks));
 #pragma unroll
           for (int nt = 0; nt < G::kNT; ++nt) mma16816<kQkBf16>(s[g][nt], r[0], r[1], r[2], r[3], qf[nt][ks][0], qf[nt][ks][1]);
         }
       }
     }
-    // scale, mask, column maxima
-    float next[G::kNT][2];
-#pragma unroll
-    for (int nt = 0; nt < G::kNT; ++nt) next[nt][0] = top[nt][0], next[nt][1] = top[nt][1];
+    // scores; the reference of the exponentials moves only when one exceeds it by 2^8
+    bool above = false;
 #pragma unroll
     for (int g = 0; g < G::kTiles; ++g) {
-      const unsigned bits = mask[g / 2] >> (g % 2 * 16);
-      const bool ok0 = (bits >> l4) & 1, ok1 = (bits >> (l4 + 8)) & 1;
-      float k0 = 1.0f, k1 = 1.0f;
-      if constexpr (INT8) k0 = ksc[g * 16 + l4], k1 = ksc[g * 16 + l4 + 8];
+      float k0 = qscale, k1 = qscale;
+      if constexpr (INT8) k0 *= ksc[g * group_gap + l4], k1 *= ksc[g * group_gap + l4 + 8];
 #pragma unroll
       for (int nt = 0; nt < G::kNT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x0 = s[g][nt][e], x1 = s[g][nt][2 + e];
-          if constexpr (INT8) x0 *= k0, x1 *= k1;
-          x0 = ok0 ? x0 * qscale[nt][e] : -INFINITY;
-          x1 = ok1 ? x1 * qscale[nt][e] : -INFINITY;
-          s[g][nt][e] = x0;
-          s[g][nt][2 + e] = x1;
-          next[nt][e] = fmaxf(next[nt][e], fmaxf(x0, x1));
+          s[g][nt][e] *= k0;
+          s[g][nt][2 + e] *= k1;
         }
     }
-    bool moved = false;
+    if (partial) {
+#pragma unroll
+      for (int g = 0; g < G::kTiles; ++g) {
+        const unsigned bits = valid[g / 2] >> (g % 2 * 16);
+#pragma unroll
+        for (int nt = 0; nt < G::kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(bits >> (l4 + (e < 2 ? 0 : 8)) & 1)) s[g][nt][e] = -INFINITY;
+      }
+    }
+    float most[G::kNT][2];
 #pragma unroll
     for (int nt = 0; nt < G::kNT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        most[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) next[nt][e] = fmaxf(next[nt][e], __shfl_xor_sync(0xFFFFFFFFu, next[nt][e], o));
-        moved |= next[nt][e] != top[nt][e];
+        for (int g = 1; g < G::kTiles; ++g) most[nt][e] = fmaxf(most[nt][e], fmaxf(s[g][nt][e], s[g][nt][2 + e]));
+        above |= most[nt][e] > top[nt][e] + kSlack;
       }
-    if (__any_sync(0xFFFFFFFFu, moved)) {
+    if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
       for (int nt = 0; nt < G::kNT; ++nt) {
-        const float f0 = ex2(top[nt][0] - next[nt][0]), f1 = ex2(top[nt][1] - next[nt][1]);
-        sum[nt][0] *= f0, sum[nt][1] *= f1;
+        float f[2];
 #pragma unroll
-        for (int m = 0; m < D / 16; ++m) acc[m][nt][0] *= f0, acc[m][nt][1] *= f1, acc[m][nt][2] *= f0, acc[m][nt][3] *= f1;
-        top[nt][0] = next[nt][0], top[nt][1] = next[nt][1];
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(most[nt][e], top[nt][e]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
+          f[e] = ex2(top[nt][e] - x);
+          top[nt][e] = x;
+          sum[nt][e] *= f[e];
+        }
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) acc[m][nt][0] *= f[0], acc[m][nt][1] *= f[1], acc[m][nt][2] *= f[0], acc[m][nt][3] *= f[1];
       }
     }
-    // weights and the second product, 16 keys at a time
+    // weights, times the values' scales
+#pragma unroll
+    for (int g = 0; g < G::kTiles; ++g) {
+      float v0 = 1.0f, v1 = 1.0f;
+      if constexpr (INT8) v0 = vsc[g * group_gap + l4], v1 = vsc[g * group_gap + l4 + 8];
+#pragma unroll
+      for (int nt = 0; nt < G::kNT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p0 = ex2(s[g][nt][e] - top[nt][e]), p1 = ex2(s[g][nt][2 + e] - top[nt][e]);
+          sum[nt][e] += p0 + p1;
+          s[g][nt][e] = INT8 ? p0 * v0 : p0;
+          s[g][nt][2 + e] = INT8 ? p1 * v1 : p1;
+        }
+    }
+    if (INT8 && partial) {                          // a scale past the length may be anything
+#pragma unroll
+      for (int g = 0; g < G::kTiles; ++g) {
+        const unsigned bits = valid[g / 2] >> (g % 2 * 16);
+#pragma unroll
+        for (int nt = 0; nt < G::kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(bits >> (l4 + (e < 2 ? 0 : 8)) & 1)) s[g][nt][e] = 0.0f;
+      }
+    }
+    // the second product, 16 keys at a time
 #pragma unroll
     for (int g = 0; g < G::kTiles; ++g) {
       uint32_t hi[G::kNT][2], lo[G::kNT][2];
-      float v0 = 1.0f, v1 = 1.0f;
-      if constexpr (INT8) v0 = ksc[G::kKeys + g * 16 + l4], v1 = ksc[G::kKeys + g * 16 + l4 + 8];
 #pragma unroll
       for (int nt = 0; nt < G::kNT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float p0 = ex2(s[g][nt][2 * h] - top[nt][0]), p1 = ex2(s[g][nt][2 * h + 1] - top[nt][1]);
-          sum[nt][0] += p0, sum[nt][1] += p1;
-          if constexpr (INT8) p0 *= h ? v1 : v0, p1 *= h ? v1 : v0;
+          const float p0 = s[g][nt][2 * h], p1 = s[g][nt][2 * h + 1];
           uint32_t w = pack2<kPvBf16>(p0, p1);
           const float2 f = unpack2<kPvBf16>(w);
           const uint32_t rest = pack2<kPvBf16>(p0 - f.x, p1 - f.y);
@@ -474,15 +593,16 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
           }
         }
       if constexpr (INT8) {
-        const int vrow = g * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
           uint32_t r[4];
-          ldsm4_t(r, swizzled(vbase, vrow, c + (lane >> 4)));
+          ldsm4_t(r, cell(vrow, g, c));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) r[x] ^= 0x80808080u;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t a0 = s8_to_bf16<0x4240>(r[2 * x]), a1 = s8_to_bf16<0x4341>(r[2 * x]);
-            const uint32_t a2 = s8_to_bf16<0x4240>(r[2 * x + 1]), a3 = s8_to_bf16<0x4341>(r[2 * x + 1]);
+            const uint32_t a0 = s8_to_bf16_64th<0x4240>(r[2 * x]), a1 = s8_to_bf16_64th<0x4341>(r[2 * x]);
+            const uint32_t a2 = s8_to_bf16_64th<0x4240>(r[2 * x + 1]), a3 = s8_to_bf16_64th<0x4341>(r[2 * x + 1]);
 #pragma unroll
             for (int nt = 0; nt < G::kNT; ++nt) {
               mma16816<true>(acc[c + x][nt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
@@ -491,11 +611,10 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
           }
         }
       } else {
-        const int vrow = g * 16 + (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
         for (int m = 0; m < D / 16; ++m) {
           uint32_t r[4];
-          ldsm4_t(r, swizzled(vbase, vrow, 2 * m + ((lane >> 3) & 1)));
+          ldsm4_t(r, cell(vrow, g, 2 * m));
 #pragma unroll
           for (int nt = 0; nt < G::kNT; ++nt) {
             mma16816<kPvBf16>(acc[m][nt], r[0], r[1], r[2], r[3], hi[nt][0], hi[nt][1]);
@@ -507,10 +626,11 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
   };
 
   // ---- end of a row's units in this CTA: join the warps, then the CTAs
-  auto out_slot = [&](int w, int slot) { return reinterpret_cast<float*>(smem + (w * kStages + slot) * G::kSlot); };
-  auto finish_row = [&](long long unit, int slot) {
-    const int kvh = at.r / a.blocks, first = kvh * a.group + (at.r % a.blocks) * HB;
-    const int n = min(HB, (kvh + 1) * a.group - first);
+  auto out_slot = [&](int w, int slot) { return reinterpret_cast<float*>(smem + (w * kStages + slot) * G::kKV); };
+  // element d of a column, spread over the banks by the column
+  auto spread = [](int col, int d) { return col * D + (d ^ ((col >> 1 & 3) << (INT8 ? 4 : 3))); };
+  auto finish_row = [&](long long index, int slot) {
+    const int first = at.head * a.group + at.block * HB, n = min(HB, a.group - at.block * HB);
     __syncwarp();
     float* o = out_slot(warp, slot);
 #pragma unroll
@@ -529,13 +649,13 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
 #pragma unroll
           for (int m = 0; m < D / 16; ++m) {
             const int d0 = INT8 ? m * 16 + 2 * l4 : m * 16 + l4, d1 = INT8 ? d0 + 1 : d0 + 8;
-            o[col * G::kOutRow + d0] = acc[m][nt][e];
-            o[col * G::kOutRow + d1] = acc[m][nt][2 + e];
+            o[spread(col, d0)] = INT8 ? acc[m][nt][e] * 64.0f : acc[m][nt][e];
+            o[spread(col, d1)] = INT8 ? acc[m][nt][2 + e] * 64.0f : acc[m][nt][2 + e];
           }
         }
       }
     __syncthreads();
-    const long long row_first = unit - at.i;
+    const long long row_first = index - at.i;
     const long long c0 = unit_owner(row_first, total, ctas), c1 = unit_owner(row_first + at.units - 1, total, ctas);
     bool joined = false;                            // the slots hold joined partials of other CTAs (no second copy)
     if (c0 != c1) {
@@ -550,11 +670,11 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float f = ex2(s_max[w * G::kCols + col] - m);
-          const float* x = out_slot(w, slot) + col * G::kOutRow + d;
+          const float* x = out_slot(w, slot) + spread(col, d);
           const float4 y = *reinterpret_cast<const float4*>(x);
           v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
           if constexpr (G::kDup) {
-            const float4 z = *reinterpret_cast<const float4*>(x + 4 * G::kOutRow);
+            const float4 z = *reinterpret_cast<const float4*>(out_slot(w, slot) + spread(col + 4, d));
             v.x += f * z.x, v.y += f * z.y, v.z += f * z.z, v.w += f * z.w;
           }
           l += f * s_sum[w * G::kCols + col];
@@ -593,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
           l = l * f + pl * g;
           m = nm;
         }
-        *reinterpret_cast<float4*>(mine_o + col * G::kOutRow + d) = v;
+        *reinterpret_cast<float4*>(mine_o + spread(col, d)) = v;
         if (d == 0) {
           s_max[warp * G::kCols + col] = m;
           s_sum[warp * G::kCols + col] = l;
@@ -611,11 +731,11 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = ex2(s_max[w * G::kCols + col] - m);
-        const float* x = out_slot(w, slot) + col * G::kOutRow + d;
+        const float* x = out_slot(w, slot) + spread(col, d);
         const float4 y = *reinterpret_cast<const float4*>(x);
         v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
         if (G::kDup && !joined) {
-          const float4 z = *reinterpret_cast<const float4*>(x + 4 * G::kOutRow);
+          const float4 z = *reinterpret_cast<const float4*>(out_slot(w, slot) + spread(col + 4, d));
           v.x += f * z.x, v.y += f * z.y, v.z += f * z.z, v.w += f * z.w;
         }
         l += f * s_sum[w * G::kCols + col];
@@ -631,61 +751,99 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kSmem <= 113 * 102
 
   // ---- main loop
   const int count = static_cast<int>(hi - lo);
-  int fetched = 0;
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (fetched < count) {
-      fetch(s);
-      ++fetched;
-      if (fetched < count) advance(in);
-    }
-    cp_async_commit();
+  look_up();
+  fetch(0);
+  if (count > 1) {
+    advance(in);
+    look_up();
   }
-  int slot = 0, fill = kStages - 1;
+  int slot = 0;
   bool fresh = true;
-  for (int u = 0; u < count; ++u) {
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    if (fetched < count) {
-      fetch(fill);
-      ++fetched;
-      if (fetched < count) advance(in);
+  for (int u = 0; u < count; ++u, slot ^= 1) {
+    if (u + 1 < count && !__any_sync(0xFFFFFFFFu, dead)) {
+      fetch(slot ^ 1);
+      if (u + 2 < count) {
+        advance(in);
+        look_up();
+      }
     }
-    cp_async_commit();
     if (fresh) start_row();
     compute(slot);
     fresh = at.i + 1 == at.units || u + 1 == count;
     if (fresh) {
       finish_row(lo + u, slot);
+      fence_proxy_async_smem();                     // the slots were written as plain memory; copies follow
       __syncthreads();
     }
     if (u + 1 < count) advance(at);
-    slot = slot + 1 == kStages ? 0 : slot + 1;
-    fill = fill + 1 == kStages ? 0 : fill + 1;
   }
 }
 
-template <bool INT8, int D, int HB>
-constexpr int resident() { return 228 * 1024 / (Geo<INT8, D, HB>::kSmem + 1024); }
+// Tensor maps of K and V with boxes of as many rows as divide a page, at most `keys`;
+// returns the rows of a box, or 0 where the lanes have to copy: pages that are no
+// multiple of 8 tokens (a box of fewer rows would split a swizzle pattern) or, in int8,
+// of 16 (the unit in which the scales are laid out), and scales that TMA cannot take.
+int make_maps(const AttnArgs& a, AttnMaps& maps, int head_dim, int elem, int span, int keys) {
+  const int least = elem == 1 ? 16 : 8;
+  int box = keys;
+  while (box >= least && a.kv.page_size % box) box /= 2;
+  if (box < least) return 0;
+  const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+  if (!encode) return 0;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(a.kv.page_size),
+                              static_cast<cuuint64_t>(a.kv.kv_heads), static_cast<cuuint64_t>(a.kv.pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.kv.token_stride * elem), static_cast<cuuint64_t>(a.kv.head_stride * elem),
+                                 static_cast<cuuint64_t>(a.kv.page_stride * elem)};
+  const cuuint32_t tile[4] = {static_cast<cuuint32_t>(span / elem), static_cast<cuuint32_t>(box), 1, 1};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 2; ++i) {
+    if (encode(i ? &maps.v : &maps.k, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4,
+               i ? a.kv.v : a.kv.k, dims, strides, tile, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return 0;
+  }
+  if (elem == 1) {
+    if (a.kv.s_token_stride != 1) return 0;
+    const cuuint64_t s_strides[2] = {static_cast<cuuint64_t>(a.kv.s_head_stride * 4), static_cast<cuuint64_t>(a.kv.s_page_stride * 4)};
+    const cuuint32_t s_tile[3] = {static_cast<cuuint32_t>(box), 1, 1};
+    for (int i = 0; i < 2; ++i) {
+      if (encode(i ? &maps.vs : &maps.ks, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, i ? a.kv.vs : a.kv.ks, dims + 1, s_strides, s_tile, ones,
+                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return 0;
+    }
+  }
+  return box;
+}
 
 template <typename T, bool INT8, int D, int HB>
-cudaError_t attn_hb(const AttnArgs& a, int sm_count, cudaStream_t s) {
+cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   using G = Geo<INT8, D, HB>;
-  // per device and instantiation: allow the shared memory
-  cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, INT8, D, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+  AttnMaps maps;
+  a.box = make_maps(a, maps, D, G::kElem, G::kSpan, G::kKeys);
+  // once per device: allow the shared memory
+  static std::atomic<unsigned long long> allowed{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (!(allowed.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(attn_kernel<T, INT8, D, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem);
+    if (e != cudaSuccess) return e;
+    allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+  }
   const long long room = static_cast<long long>(a.columns) * a.kv.page_size;
   const long long most = static_cast<long long>(a.batch) * a.kv.kv_heads * a.blocks * ((room + G::kUnit - 1) / G::kUnit);
-  const long long wave = static_cast<long long>(sm_count) * resident<INT8, D, HB>();
+  const long long wave = static_cast<long long>(sm_count) * G::kResident;
   const unsigned grid = static_cast<unsigned>(std::max(1ll, std::min(most, wave)));
-  attn_kernel<T, INT8, D, HB><<<grid, kThreads, G::kSmem, s>>>(a);
+  attn_kernel<T, INT8, D, HB><<<grid, kThreads, G::kSmem, s>>>(a, maps);
   return cudaGetLastError();
 }
 
 int heads_per_cta(int group, int head_dim) { return group <= 4 ? 4 : group <= 8 || head_dim == 256 ? 8 : 16; }
 
 template <typename T, bool INT8, int D>
-cudaError_t attn_d(const AttnArgs& a, int sm_count, cudaStream_t s) {
+cudaError_t attn_d(AttnArgs& a, int sm_count, cudaStream_t s) {
   const int hb = heads_per_cta(a.group, D);
   if (hb == 4) return attn_hb<T, INT8, D, 4>(a, sm_count, s);
   if constexpr (D != 256)
@@ -694,7 +852,7 @@ cudaError_t attn_d(const AttnArgs& a, int sm_count, cudaStream_t s) {
 }
 
 template <typename T, bool INT8>
-cudaError_t attn_t(const AttnArgs& a, int head_dim, int sm_count, cudaStream_t s) {
+cudaError_t attn_t(AttnArgs& a, int head_dim, int sm_count, cudaStream_t s) {
   return head_dim == 64    ? attn_d<T, INT8, 64>(a, sm_count, s)
          : head_dim == 128 ? attn_d<T, INT8, 128>(a, sm_count, s)
                            : attn_d<T, INT8, 256>(a, sm_count, s);
@@ -706,7 +864,7 @@ size_t paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int h
   // two partial rows per CTA of the widest wave
   (void)batch;
   const int hb = heads_per_cta(heads / std::max(1, kv_heads), head_dim);
-  return kCounterBytes + 2ull * 2 * sm_count * hb * (head_dim + 2) * sizeof(float);
+  return kCounterBytes + 2ull * 3 * sm_count * hb * (head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int heads, long long q_row_stride,
@@ -728,6 +886,10 @@ cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int head
   const int hb = heads_per_cta(a.group, cache.head_dim);
   a.blocks = (a.group + hb - 1) / hb;
   a.q_vec = (reinterpret_cast<uintptr_t>(q) % 4 == 0) && q_row_stride % 2 == 0 && q_head_stride % 2 == 0;
+  int log = 0;
+  while ((1ll << log) < cache.page_size) ++log;
+  a.page_mul = static_cast<uint32_t>(((1ull << (31 + log)) + cache.page_size - 1) / cache.page_size);
+  a.page_shift = 31 + log;
   a.scale = scale;
   a.out = out;
   a.lse = lse;

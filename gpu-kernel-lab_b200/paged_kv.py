@@ -27,6 +27,7 @@ The functions are for inference: tensors that require grad are refused, as
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -98,17 +99,31 @@ def _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype):
 
 
 def _check_vector(t, name, dtype, count, device):
-    if t.shape != (count,) or t.dtype != dtype or not t.is_contiguous() or t.device != device:
+    if t.dtype != dtype or t.shape != (count,) or t.device != device or not t.is_contiguous():
         raise ValueError(f'{name} must be a contiguous {dtype} vector of {count} on the cache\'s device')
+
+
+def _output(q):
+    """An uninitialised contiguous tensor like ``q``."""
+    return torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
 
 
 def _call(device, fn, *args):
     """``fn(*args, stream)`` with ``device`` current."""
-    if device.index == torch.cuda.current_device():
-        N.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            N.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        N.check(status)
+
+
+@functools.lru_cache(maxsize=256)
+def paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim) -> int:
+    """Bytes of scratch that ``paged_attention`` needs, for a ``workspace`` of the caller's own."""
+    return N.lib().kl_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim)
 
 
 def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales=None, v_scales=None,
@@ -153,7 +168,7 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
     _check_vector(slots, 'slots', torch.int64, tokens, device)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise ValueError('inference only; use torch.inference_mode()')
-    out = torch.empty((tokens, heads, dim), dtype=dtype, device=device)
+    out = _output(q)
     if tokens:
         _call(device, N.lib().kl_qk_norm_rope_write, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0],
               sv[1], _CODES[dtype], tokens, heads, None if q_weight is None else q_weight.data_ptr(),
@@ -175,7 +190,8 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
     device, tokens = k_cache.device, slots.numel()
     _check_vector(slots, 'slots', torch.int64, tokens, device)
     shape = (tokens, k_cache.shape[1], k_cache.shape[3])
-    k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    k = torch.empty(shape, dtype=dtype, device=device)
+    v = torch.empty_like(k)
     if tokens:
         _call(device, N.lib().kl_read_kv, cache, _CODES[dtype], slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
     return k, v
@@ -222,22 +238,15 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
         raise ValueError('scale must be finite')
     if torch.is_grad_enabled() and q.requires_grad:
         raise ValueError('inference only; use torch.inference_mode()')
-    out = torch.empty((batch, heads, dim), dtype=dtype, device=device)
+    out = _output(q)
     lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
     if batch:
-        lib = N.lib()
         if workspace is None:
-            need = lib.kl_paged_attention_workspace_bytes(batch, heads, kv_heads, dim)
-            workspace = N.workspace(device, need, stream=torch.cuda.current_stream(device))
+            workspace = N.workspace(device, paged_attention_workspace_bytes(1, heads, kv_heads, dim),
+                                    torch._C._cuda_getCurrentRawStream(device.index))
         elif workspace.device != device or not workspace.is_contiguous():
             raise ValueError('workspace must be contiguous, on the cache\'s device')
-        _call(device, lib.kl_paged_attention, q.data_ptr(), strides[0], strides[1], _CODES[dtype], batch, heads, cache,
+        _call(device, N.lib().kl_paged_attention, q.data_ptr(), strides[0], strides[1], _CODES[dtype], batch, heads, cache,
               page_table.data_ptr(), table_stride, columns, lengths.data_ptr(), scale, out.data_ptr(),
-              None if lse is None else lse.data_ptr(), None if workspace is None else workspace.data_ptr(),
-              0 if workspace is None else workspace.numel() * workspace.element_size())
+              None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return (out, lse) if return_lse else out
-
-
-def paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim) -> int:
-    """Bytes of scratch that ``paged_attention`` needs, for a ``workspace`` of the caller's own."""
-    return N.lib().kl_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim)
