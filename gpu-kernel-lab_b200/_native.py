@@ -156,6 +156,10 @@ def workspace(device: torch.device, nbytes: int, stream=None) -> torch.Tensor | 
     if nbytes == 0:
         return None
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    if type(stream) is int and stream == 0:          # the default stream, which is never captured
+        buf = _workspaces.get(idx)
+        if buf is not None and buf.numel() >= nbytes:
+            return buf
     capturing = torch.cuda.is_current_stream_capturing()
     key = idx
     if stream is not None and not capturing:

@@ -974,6 +974,9 @@ int kl_paged_attention(const void* q, long long q_row_stride, long long q_head_s
   if (!aligned16(out)) return fail(KL_ERR_INVALID, "out must be 16-byte aligned");
   if (static_cast<long long>(columns) * cache->page_size > 0x7FFF0000ll || static_cast<long long>(batch) * heads > 0x7FFFFFFFll)
     return fail(KL_ERR_INVALID, "columns * page_size and batch * heads must stay below 2^31");
+  // units of at least 64 keys; the kernel counts them in 32 bits
+  if (static_cast<long long>(batch) * heads * ((static_cast<long long>(columns) * cache->page_size + 63) / 64) > 0x7FFFFFFFll)
+    return fail(KL_ERR_INVALID, "batch * heads * columns * page_size / 64 must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
   const size_t need = paged_attention_workspace_bytes(batch, heads, cache->kv_heads, cache->head_dim, di.sm_count);

@@ -43,10 +43,21 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 2;
+constexpr int kMaxCtas = 640;          // bound of the grid: 3 per SM of up to 213 SMs
+constexpr int kMaxPrefetch = 16384;    // 128-byte lines
+constexpr int kRecordBytes = 16 * 1024;
+constexpr int kJoinThreads = 512;
+constexpr int kWholeUnits = 4;         // rows of up to so many units are not split
 constexpr int kMaxLens = 512;          // lengths kept in shared memory
 constexpr float kSlack = 8.0f;           // log2 of how far weights may exceed 1
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
+// A row that several CTAs have parts of, as its first CTA records it
+struct Piece {
+  int ways;                            // CTAs of the row; 0: the CTA begins no such row
+  int heads, row;                      // heads of the row, and the first one's place in the output
+};
 
 struct AttnArgs {
   const void* q;
@@ -65,8 +76,9 @@ struct AttnArgs {
   float scale;
   void* out;
   float* lse;
-  int* counters;
-  float* partials;
+  Piece* records;                      // one per CTA; null: rows are not split
+  float* partials;                     // two per CTA
+  void* workspace;
   int* status;
 };
 
@@ -88,6 +100,8 @@ KL_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, i
 KL_DEVICE void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(bar) : "memory");
 }
+
+KL_DEVICE void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" :: "l"(p)); }
 
 KL_DEVICE float ex2(float x) {
   float y;
@@ -169,7 +183,7 @@ struct Geo {
   static constexpr int kScales = kTiles * 128;                    // bytes for a slot's key (or value) scales
   static constexpr int kNote = (INT8 ? 2 * kScales : 0) + 128;    // per slot: the scales, and the mask of the valid keys
   static constexpr int kStats = 2 * kWarps * kCols * 4;           // every warp's maximum and sum per column
-  static constexpr int kSmem = 1024 + kRing + kWarps * kStages * (kNote + 8) + kStats + kMaxLens * 4 + 64;
+  static constexpr int kSmem = 1024 + kRing + kWarps * kStages * (kNote + 8) + kStats + kMaxLens * 4 + 96;
   static constexpr int kResident = kSmem > 113 * 1024 ? 1 : HB == 16 || D == 256 ? 2 : 3;   // CTAs per SM
   static_assert(kCols * D * 4 <= kKV, "a warp's output goes over its consumed slot");
   static constexpr int kPartial = HB * (D + 2);                   // floats of one partial row
@@ -180,6 +194,15 @@ struct Cursor {
   int b, head, block, i;   // sequence, KV head, block of its query heads, unit of that row
   int units, len;
 };
+
+// Four output elements of one head from their weighted sum v, the reference m and the weights' sum l
+template <bool BF16, int D, typename T>
+KL_DEVICE void emit(T* out, float* lse, int row, int d, float4 v, float m, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<uint2*>(out + static_cast<size_t>(row) * D + d) =
+      make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+  if (d == 0 && lse) lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
 
 template <typename T, bool INT8, int D, int HB>
 __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
@@ -198,11 +221,34 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   float* s_max = reinterpret_cast<float*>(bars + kWarps * kStages);
   float* s_sum = s_max + kWarps * G::kCols;
   int* s_len = reinterpret_cast<int*>(s_sum + kWarps * G::kCols);
-  int* s_misc = s_len + kMaxLens;                   // [0..7] scan totals, [8] start b, [9] start rest, [10] last flag
+  int* s_misc = s_len + kMaxLens;                   // [0..3] scan totals, [8] start b, [9] start rest, [10] end b, [11] end rest
+  Piece* s_piece = reinterpret_cast<Piece*>(s_misc + 12);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int t4 = lane & 3, l4 = lane >> 2;
   const int rows = a.kv.kv_heads * a.blocks;        // rows per sequence
+
+  pdl_launch_dependents();                          // the join's blocks wait for this grid's end by themselves
+
+  // ---- what the first unit will wait for is brought into L2 while the lengths are read
+  if (tid == 0) {
+    prefetch_tmap(&maps.k);
+    prefetch_tmap(&maps.v);
+    if constexpr (INT8) {
+      prefetch_tmap(&maps.ks);
+      prefetch_tmap(&maps.vs);
+    }
+  }
+  {
+    const int row_lines = (a.columns + 31) / 32, head_lines = D * 2 / 128;
+    const long long table_lines = static_cast<long long>(a.batch) * row_lines, q_lines = static_cast<long long>(a.batch) * a.heads * head_lines;
+    for (int i = blockIdx.x * kThreads + tid; i < min(table_lines, static_cast<long long>(kMaxPrefetch)); i += gridDim.x * kThreads)
+      prefetch_l2(a.table + i / row_lines * a.table_stride + i % row_lines * 32);
+    for (int i = blockIdx.x * kThreads + tid; i < min(q_lines, static_cast<long long>(kMaxPrefetch)); i += gridDim.x * kThreads) {
+      const int h = i / head_lines;
+      prefetch_l2(static_cast<const char*>(a.q) + (h / a.heads * a.q_row_stride + h % a.heads * a.q_head_stride) * 2 + i % head_lines * 128);
+    }
+  }
 
   // ---- this CTA's units: one scan over the sequences' unit counts
   const long long room = static_cast<long long>(a.columns) * a.kv.page_size;
@@ -213,32 +259,33 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   auto units_of = [&](int n) { return (n + G::kUnit - 1) / G::kUnit; };
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-  long long mine = 0;
+  int mine = 0;
   for (int b = b0; b < b1; ++b) {
     const int n = length_of(b);
     if (a.lengths[b] > room) record_error(a.status, KL_ERR_INVALID);
     if (b < kMaxLens) s_len[b] = n;
     mine += units_of(n);
   }
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
     if (lane >= o) incl += v;
   }
-  long long* s_tot = reinterpret_cast<long long*>(s_misc);
+  int* s_tot = s_misc;
   if (lane == 31) s_tot[warp] = incl;
   if (tid < kWarps * kStages) mbar_init(smem_u32(bars + tid), a.box ? 1 : 33);
   if (tid == 0) fence_mbar_init();
+  if (tid == 0) s_piece->ways = 0;
   __syncthreads();
-  long long total = 0;
+  int total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) incl += s_tot[w];
     total += s_tot[w];
   }
   total *= rows;
-  const long long ctas = total < static_cast<long long>(gridDim.x) ? total : gridDim.x;
+  const int ctas = min(total, static_cast<int>(gridDim.x));
   // sequences without tokens: zeros
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     if ((b < kMaxLens ? s_len[b] : length_of(b)) > 0) continue;
@@ -247,18 +294,28 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     if (a.lse)
       for (int i = tid; i < a.heads; i += kThreads) a.lse[static_cast<size_t>(b) * a.heads + i] = -INFINITY;
   }
-  if (blockIdx.x >= ctas) return;
-  const long long lo = unit_lo(blockIdx.x, total, ctas), hi = unit_lo(blockIdx.x + 1, total, ctas);
-  if ((incl - mine) * rows <= lo && lo < incl * rows) {
-    long long before = (incl - mine) * rows;
-    int b = b0;
-    for (;; ++b) {
-      const long long u = static_cast<long long>(units_of(length_of(b))) * rows;
-      if (lo < before + u) break;
-      before += u;
+  if (blockIdx.x >= ctas) {
+    if (tid == 0 && a.records) a.records[blockIdx.x].ways = 0;
+    return;
+  }
+  // CTA c has units [lo(c), lo(c + 1)): share + 1 each in the first `more` CTAs, share in the others
+  const int share = total / ctas, more = total - share * ctas, cta = blockIdx.x;
+  const int lo = cta * share + min(cta, more), hi = lo + share + (cta < more ? 1 : 0);
+  auto owner = [&](int u) { return u < more * (share + 1) ? u / (share + 1) : more + (u - more * (share + 1)) / share; };
+  // the sequences of the first unit and of the one past the last
+#pragma unroll
+  for (int end = 0; end < 2; ++end) {
+    const int u = end ? hi : lo;
+    if ((incl - mine) * rows <= u && u < incl * rows) {
+      int before = (incl - mine) * rows, b = b0;
+      for (;; ++b) {
+        const int n = units_of(length_of(b)) * rows;
+        if (u < before + n) break;
+        before += n;
+      }
+      s_misc[8 + 2 * end] = b;
+      s_misc[9 + 2 * end] = u - before;
     }
-    s_misc[8] = b;
-    s_misc[9] = static_cast<int>(lo - before);
   }
   __syncthreads();
   auto load_len = [&](Cursor& c) {
@@ -277,12 +334,25 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
       load_len(c);
     } while (c.units == 0);
   };
+  int count = hi - lo;
   Cursor in;                                        // next unit to fetch
   in.b = s_misc[8];
   load_len(in);
   in.i = s_misc[9] % in.units;
   in.head = s_misc[9] / in.units / a.blocks;
   in.block = s_misc[9] / in.units % a.blocks;
+  if (!a.records) {                                 // whole rows: those that begin in [lo, hi)
+    if (hi < total) {
+      const int units = units_of(s_misc[10] < kMaxLens ? s_len[s_misc[10]] : length_of(s_misc[10])), over = s_misc[11] % units;
+      if (over) count += units - over;
+    }
+    if (in.i > 0) {
+      count -= in.units - in.i;
+      in.i = in.units - 1;
+      if (count > 0) advance(in);
+    }
+    if (count <= 0) return;
+  }
   Cursor at = in;                                   // unit being computed
 
   // ---- fetching: this warp's keys of the unit `in` into ring slot `slot`
@@ -629,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   auto out_slot = [&](int w, int slot) { return reinterpret_cast<float*>(smem + (w * kStages + slot) * G::kKV); };
   // element d of a column, spread over the banks by the column
   auto spread = [](int col, int d) { return col * D + (d ^ ((col >> 1 & 3) << (INT8 ? 4 : 3))); };
-  auto finish_row = [&](long long index, int slot) {
+  auto finish_row = [&](int index, int slot) {
     const int first = at.head * a.group + at.block * HB, n = min(HB, a.group - at.block * HB);
     __syncwarp();
     float* o = out_slot(warp, slot);
@@ -655,102 +725,41 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
         }
       }
     __syncthreads();
-    const long long row_first = index - at.i;
-    const long long c0 = unit_owner(row_first, total, ctas), c1 = unit_owner(row_first + at.units - 1, total, ctas);
-    bool joined = false;                            // the slots hold joined partials of other CTAs (no second copy)
-    if (c0 != c1) {
-      float* part = a.partials + (blockIdx.x * 2ll + (blockIdx.x == c0 ? 1 : 0)) * G::kPartial;
-      for (int i = tid; i < n * (D / 4); i += kThreads) {
-        const int col = i / (D / 4), d = i % (D / 4) * 4;
-        float m = -FLT_MAX;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_max[w * G::kCols + col]);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = ex2(s_max[w * G::kCols + col] - m);
-          const float* x = out_slot(w, slot) + spread(col, d);
-          const float4 y = *reinterpret_cast<const float4*>(x);
-          v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
-          if constexpr (G::kDup) {
-            const float4 z = *reinterpret_cast<const float4*>(out_slot(w, slot) + spread(col + 4, d));
-            v.x += f * z.x, v.y += f * z.y, v.z += f * z.z, v.w += f * z.w;
-          }
-          l += f * s_sum[w * G::kCols + col];
-        }
-        *reinterpret_cast<float4*>(part + col * D + d) = v;
-        if (d == 0) {
-          part[HB * D + col] = m;
-          part[HB * D + HB + col] = l;
-        }
-      }
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const int count = static_cast<int>(c1 - c0 + 1);
-        const int seen = atomicAdd(a.counters + c0, 1);
-        if (seen == count - 1) a.counters[c0] = 0;
-        s_misc[10] = seen == count - 1;
-      }
-      __syncthreads();
-      if (!s_misc[10]) return;
-      __threadfence();
-      joined = true;
-      // warp w takes the CTAs c0 + w, c0 + w + kWarps, ...
-      float* mine_o = out_slot(warp, slot);
-      for (int i = lane; i < n * (D / 4); i += 32) {
-        const int col = i / (D / 4), d = i % (D / 4) * 4;
-        float m = -FLT_MAX, l = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (long long c = c0 + warp; c <= c1; c += kWarps) {
-          const float* p = a.partials + (c * 2 + (c == c0 ? 1 : 0)) * G::kPartial;
-          const float pm = __ldcg(p + HB * D + col), pl = __ldcg(p + HB * D + HB + col);
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(p + col * D + d));
-          const float nm = fmaxf(m, pm), f = ex2(m - nm), g = ex2(pm - nm);
-          v.x = v.x * f + y.x * g, v.y = v.y * f + y.y * g, v.z = v.z * f + y.z * g, v.w = v.w * f + y.w * g;
-          l = l * f + pl * g;
-          m = nm;
-        }
-        *reinterpret_cast<float4*>(mine_o + spread(col, d)) = v;
-        if (d == 0) {
-          s_max[warp * G::kCols + col] = m;
-          s_sum[warp * G::kCols + col] = l;
-        }
-      }
-      __syncthreads();
-    }
-    const size_t row = static_cast<size_t>(at.b) * a.heads + first;
+    const int row = at.b * a.heads + first;
+    const int row_first = index - at.i, c0 = a.records ? owner(row_first) : cta, c1 = a.records ? owner(row_first + at.units - 1) : cta;
+    const int ways = c1 - c0 + 1, own = cta - c0;
     for (int i = tid; i < n * (D / 4); i += kThreads) {
       const int col = i / (D / 4), d = i % (D / 4) * 4;
       float m = -FLT_MAX, l = 0.0f;
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_max[w * G::kCols + col]);
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = ex2(s_max[w * G::kCols + col] - m);
-        const float* x = out_slot(w, slot) + spread(col, d);
-        const float4 y = *reinterpret_cast<const float4*>(x);
+        const float4 y = *reinterpret_cast<const float4*>(out_slot(w, slot) + spread(col, d));
         v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
-        if (G::kDup && !joined) {
+        if constexpr (G::kDup) {
           const float4 z = *reinterpret_cast<const float4*>(out_slot(w, slot) + spread(col + 4, d));
           v.x += f * z.x, v.y += f * z.y, v.z += f * z.z, v.w += f * z.w;
         }
         l += f * s_sum[w * G::kCols + col];
       }
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint2 packed;
-      packed.x = pack2<kBf16>(v.x * inv, v.y * inv);
-      packed.y = pack2<kBf16>(v.z * inv, v.w * inv);
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row + col) * D + d) = packed;
-      if (d == 0 && a.lse) a.lse[row + col] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+      if (ways == 1) {
+        emit<kBf16, D>(static_cast<T*>(a.out), a.lse, row + col, d, v, m, l);
+      } else {
+        float* p = a.partials + static_cast<long long>(cta * 2 + (own == 0 ? 1 : 0)) * G::kPartial;
+        __stcg(reinterpret_cast<float4*>(p + col * D + d), v);
+        if (d == 0) {
+          __stcg(p + HB * D + col, m);
+          __stcg(p + HB * D + HB + col, l);
+        }
+      }
     }
+    if (ways > 1 && own == 0 && tid == 0) *s_piece = {ways, n, row};
   };
 
   // ---- main loop
-  const int count = static_cast<int>(hi - lo);
   look_up();
   fetch(0);
   if (count > 1) {
@@ -777,6 +786,71 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     }
     if (u + 1 < count) advance(at);
   }
+
+  if (tid == 0 && a.records) a.records[cta] = *s_piece;
+}
+
+// The rows that several CTAs have parts of: block (c, y) joins four heads of the row whose
+// first part is CTA c's. Launched behind the attention kernel as its programmatic dependent.
+// One block that joined a row inside that kernel, after an atomic arrival of each part, took
+// 8 us where this takes 3: a chain of round trips with the row's data going through one SM.
+template <typename T, int D, int HB>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Piece* records, const float* partials, T* out, float* lse) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kHeads = HB < 4 ? HB : 4, kVecs = kHeads * D / 4, kSides = kJoinThreads / kVecs;
+  __shared__ float4 s_v[kSides][kVecs];
+  __shared__ float s_m[kSides][kVecs], s_l[kSides][kVecs];
+  pdl_wait();
+  const Piece piece = records[blockIdx.x];
+  const int side = threadIdx.x / kVecs, vec = threadIdx.x % kVecs;
+  const int col = blockIdx.y * kHeads + vec / (D / 4), d = vec % (D / 4) * 4;
+  if (piece.ways == 0 || blockIdx.y * kHeads >= piece.heads) return;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -FLT_MAX, l = 0.0f;
+  if (col < piece.heads) {
+    for (int k0 = side; k0 < piece.ways; k0 += 8 * kSides) {
+      float4 y[8];
+      float pm[8], pl[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = k0 + i * kSides;
+        y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), pm[i] = -FLT_MAX, pl[i] = 0.0f;
+        if (k < piece.ways) {
+          const float* x = partials + static_cast<long long>((blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * (HB * (D + 2));
+          y[i] = __ldcg(reinterpret_cast<const float4*>(x + col * D + d));
+          pm[i] = __ldcg(x + HB * D + col);
+          pl[i] = __ldcg(x + HB * D + HB + col);
+        }
+      }
+      float most = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, pm[i]);
+      const float keep = ex2(m - most);
+      v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep, l *= keep;
+      m = most;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = ex2(pm[i] - m);
+        v.x += f * y[i].x, v.y += f * y[i].y, v.z += f * y[i].z, v.w += f * y[i].w;
+        l += f * pl[i];
+      }
+    }
+  }
+  s_v[side][vec] = v;
+  s_m[side][vec] = m;
+  s_l[side][vec] = l;
+  __syncthreads();
+  if (side > 0 || col >= piece.heads) return;
+  for (int k = 1; k < kSides; ++k) m = fmaxf(m, s_m[k][vec]);
+  v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  l = 0.0f;
+  for (int k = 0; k < kSides; ++k) {
+    const float f = ex2(s_m[k][vec] - m);
+    const float4 y = s_v[k][vec];
+    v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
+    l += f * s_l[k][vec];
+  }
+  emit<kBf16, D>(out, lse, piece.row + col, d, v, m, l);
 }
 
 // Tensor maps of K and V with boxes of as many rows as divide a page, at most `keys`;
@@ -835,9 +909,23 @@ cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   const long long room = static_cast<long long>(a.columns) * a.kv.page_size;
   const long long most = static_cast<long long>(a.batch) * a.kv.kv_heads * a.blocks * ((room + G::kUnit - 1) / G::kUnit);
   const long long wave = static_cast<long long>(sm_count) * G::kResident;
-  const unsigned grid = static_cast<unsigned>(std::max(1ll, std::min(most, wave)));
+  const unsigned grid = static_cast<unsigned>(std::max(1ll, std::min({most, wave, static_cast<long long>(kMaxCtas)})));
+  char* const space = static_cast<char*>(a.workspace) + kCounterBytes;
+  a.records = room > kWholeUnits * G::kUnit ? reinterpret_cast<Piece*>(space) : nullptr;
+  a.partials = reinterpret_cast<float*>(space + kRecordBytes);
   attn_kernel<T, INT8, D, HB><<<grid, kThreads, G::kSmem, s>>>(a, maps);
-  return cudaGetLastError();
+  if ((e = cudaGetLastError()) != cudaSuccess || !a.records) return e;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid, (std::min(a.group, HB) + 3) / 4);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, join_kernel<T, D, HB>, static_cast<const Piece*>(a.records), static_cast<const float*>(a.partials),
+                            static_cast<T*>(a.out), a.lse);
 }
 
 int heads_per_cta(int group, int head_dim) { return group <= 4 ? 4 : group <= 8 || head_dim == 256 ? 8 : 16; }
@@ -864,7 +952,7 @@ size_t paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int h
   // two partial rows per CTA of the widest wave
   (void)batch;
   const int hb = heads_per_cta(heads / std::max(1, kv_heads), head_dim);
-  return kCounterBytes + 2ull * 3 * sm_count * hb * (head_dim + 2) * sizeof(float);
+  return kCounterBytes + kRecordBytes + 2ull * std::min(3 * sm_count, kMaxCtas) * hb * (head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int heads, long long q_row_stride,
@@ -893,8 +981,7 @@ cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int head
   a.scale = scale;
   a.out = out;
   a.lse = lse;
-  a.counters = static_cast<int*>(workspace);
-  a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+  a.workspace = workspace;
   a.status = status;
   const bool int8 = cache.format == KL_KV_INT8;
   if (dtype == KL_DT_BF16)

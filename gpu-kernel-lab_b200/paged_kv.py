@@ -36,6 +36,7 @@ import torch
 from . import _native as N
 
 HEAD_DIMS = (64, 128, 256)
+_raw_stream = torch._C._cuda_getCurrentRawStream     # as an integer; torch.cuda.current_stream() takes 2 us of host time
 _CODES = {torch.bfloat16: N.KL_DT_BF16, torch.float16: N.KL_DT_F16}
 
 
@@ -66,40 +67,43 @@ def kv_slots(page_table, rows, positions, page_size):
     return page_table[rows, positions // page_size].long() * page_size + positions % page_size
 
 
-def _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype):
-    """Checks of the cache that the three operators share, and its ``kl_kv_cache``."""
-    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError('k_cache and v_cache must be [pages, kv_heads, page_size, head_dim]')
-    pages, kv_heads, page_size, head_dim = k_cache.shape
+def _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index):
+    """Checks of the cache that the three operators share, and its ``kl_kv_cache``; ``index`` is the CUDA device."""
+    shape = k_cache.shape
     strides = k_cache.stride()
+    held = k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError('k_cache and v_cache must be [pages, kv_heads, page_size, head_dim]')
     if v_cache.stride() != strides or strides[3] != 1:
         raise ValueError('k_cache and v_cache must have equal strides and contiguous head elements')
-    device = k_cache.device
-    if not k_cache.is_cuda or v_cache.device != device:
-        raise ValueError('the cache must be on one CUDA device')
+    if index < 0 or k_cache.get_device() != index or v_cache.get_device() != index:
+        raise ValueError('the cache must be on the same CUDA device as the other tensors')
+    pages, kv_heads, page_size, head_dim = shape
     if head_dim not in HEAD_DIMS:
         raise ValueError('head_dim must be 64, 128 or 256')
-    if k_cache.dtype != v_cache.dtype:
+    if v_cache.dtype != held:
         raise ValueError('k_cache and v_cache must have one dtype')
-    if k_cache.dtype == torch.int8:
+    if held == torch.int8:
         if k_scales is None or v_scales is None:
             raise ValueError('an int8 cache needs k_scales and v_scales')
-        if k_scales.shape != k_cache.shape[:3] or v_scales.shape != k_cache.shape[:3] or k_scales.stride() != v_scales.stride():
+        scale_strides = k_scales.stride()
+        if k_scales.shape != shape[:3] or v_scales.shape != shape[:3] or v_scales.stride() != scale_strides:
             raise ValueError('scales must be [pages, kv_heads, page_size] with equal strides')
-        if k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.device != device or v_scales.device != device:
+        if (k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.get_device() != index
+                or v_scales.get_device() != index):
             raise ValueError('scales must be FP32 on the cache\'s device')
-        return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), *strides[:3],
-                               *k_scales.stride(), N.KL_KV_INT8, pages, page_size, kv_heads, head_dim)
+        return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), strides[0],
+                               strides[1], strides[2], *scale_strides, N.KL_KV_INT8, pages, page_size, kv_heads, head_dim)
     if k_scales is not None or v_scales is not None:
         raise ValueError('only an int8 cache has scales')
-    if k_cache.dtype != dtype:
+    if held != dtype:
         raise ValueError('the cache must be int8 or of the activations\' dtype')
-    return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, *strides[:3], 0, 0, 0, N.KL_KV_SAME, pages, page_size,
-                           kv_heads, head_dim)
+    return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, strides[0], strides[1], strides[2], 0, 0, 0, N.KL_KV_SAME,
+                           pages, page_size, kv_heads, head_dim)
 
 
-def _check_vector(t, name, dtype, count, device):
-    if t.dtype != dtype or t.shape != (count,) or t.device != device or not t.is_contiguous():
+def _check_vector(t, name, dtype, count, index):
+    if t.dtype != dtype or t.shape != (count,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f'{name} must be a contiguous {dtype} vector of {count} on the cache\'s device')
 
 
@@ -108,14 +112,13 @@ def _output(q):
     return torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
 
 
-def _call(device, fn, *args):
-    """``fn(*args, stream)`` with ``device`` current."""
-    index = device.index
+def _call(index, fn, *args):
+    """``fn(*args, stream)`` with CUDA device ``index`` current."""
     if index == torch.cuda.current_device():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
     if status:
         N.check(status)
 
@@ -138,41 +141,44 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
 
     The arithmetic is f32 up to one rounding at the store (an int8 cache quantises the f32 value).
     """
-    if q.ndim != 3 or k.ndim != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    shape, kv_shape = q.shape, k.shape
+    if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape or shape[0] != kv_shape[0] or shape[2] != kv_shape[2]:
         raise ValueError('q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]')
-    tokens, heads, dim = q.shape
-    dtype, device = q.dtype, q.device
+    tokens, heads, dim = shape
+    dtype, index = q.dtype, q.get_device()
     if dtype not in _CODES or k.dtype != dtype or v.dtype != dtype:
         raise ValueError('q, k and v must have matching FP16/BF16 dtype')
-    if not q.is_cuda or k.device != device or v.device != device or k_cache.device != device:
+    if index < 0 or k.get_device() != index or v.get_device() != index:
         raise ValueError('q, k, v and the cache must be on the same CUDA device')
     sq, sk, sv = q.stride(), k.stride(), v.stride()
     if tokens and (sq[2] != 1 or sk[2] != 1 or sv[2] != 1):
         raise ValueError('q, k and v must have contiguous head elements')
-    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype)
-    if k.shape[1] != k_cache.shape[1] or dim != k_cache.shape[3]:
+    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index)
+    if kv_shape[1] != k_cache.shape[1] or dim != k_cache.shape[3]:
         raise ValueError('k and v must match the cache\'s heads and head_dim')
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError('q_weight and k_weight must be given together')
-    if q_weight is not None:
-        _check_vector(q_weight, 'q_weight', dtype, dim, device)
-        _check_vector(k_weight, 'k_weight', dtype, dim, device)
-        if not math.isfinite(epsilon) or epsilon <= 0:
+    q_weight_at = k_weight_at = None
+    if q_weight is not None and k_weight is not None:
+        _check_vector(q_weight, 'q_weight', dtype, dim, index)
+        _check_vector(k_weight, 'k_weight', dtype, dim, index)
+        if not 0 < epsilon < math.inf:
             raise ValueError('epsilon must be finite and positive')
-    if cos.ndim != 2 or cos.shape[0] == 0 or cos.shape[1] != dim // 2 or sin.shape != cos.shape:
+        q_weight_at, k_weight_at = q_weight.data_ptr(), k_weight.data_ptr()
+    elif q_weight is not None or k_weight is not None:
+        raise ValueError('q_weight and k_weight must be given together')
+    table = cos.shape
+    if len(table) != 2 or table[0] == 0 or 2 * table[1] != dim or sin.shape != table:
         raise ValueError('cos and sin must be [max_positions, head_dim / 2]')
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != device or sin.device != device
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.get_device() != index or sin.get_device() != index
             or not cos.is_contiguous() or not sin.is_contiguous()):
         raise ValueError('cos and sin must be contiguous FP32 on the cache\'s device')
-    _check_vector(positions, 'positions', torch.int64, tokens, device)
-    _check_vector(slots, 'slots', torch.int64, tokens, device)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    _check_vector(positions, 'positions', torch.int64, tokens, index)
+    _check_vector(slots, 'slots', torch.int64, tokens, index)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError('inference only; use torch.inference_mode()')
     out = _output(q)
     if tokens:
-        _call(device, N.lib().kl_qk_norm_rope_write, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0],
-              sv[1], _CODES[dtype], tokens, heads, None if q_weight is None else q_weight.data_ptr(),
-              None if k_weight is None else k_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        _call(index, N.lib().kl_qk_norm_rope_write, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0],
+              sv[1], _CODES[dtype], tokens, heads, q_weight_at, k_weight_at, cos.data_ptr(), sin.data_ptr(), table[0],
               positions.data_ptr(), slots.data_ptr(), epsilon, cache, out.data_ptr())
     return out
 
@@ -186,14 +192,15 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
         dtype = torch.bfloat16 if k_cache.dtype == torch.int8 else k_cache.dtype
     if dtype not in _CODES:
         raise ValueError('keys and values are read as FP16/BF16')
-    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype)
-    device, tokens = k_cache.device, slots.numel()
-    _check_vector(slots, 'slots', torch.int64, tokens, device)
+    index = slots.get_device()
+    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index)
+    tokens = slots.numel()
+    _check_vector(slots, 'slots', torch.int64, tokens, index)
     shape = (tokens, k_cache.shape[1], k_cache.shape[3])
-    k = torch.empty(shape, dtype=dtype, device=device)
+    k = k_cache.new_empty(shape, dtype=dtype)
     v = torch.empty_like(k)
     if tokens:
-        _call(device, N.lib().kl_read_kv, cache, _CODES[dtype], slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
+        _call(index, N.lib().kl_read_kv, cache, _CODES[dtype], slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -211,42 +218,43 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     exponentials (``-inf`` for a length of 0), by which parts of a sequence can be joined.  ``workspace`` (uint8, zeroed
     once, of ``paged_attention_workspace_bytes``) takes the place of the scratch kept per device and stream.
     """
-    if q.ndim != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise ValueError('q must be [batch, heads, head_dim]')
-    batch, heads, dim = q.shape
-    dtype, device = q.dtype, q.device
+    batch, heads, dim = shape
+    dtype, index = q.dtype, q.get_device()
     if dtype not in _CODES:
         raise ValueError('q must be FP16/BF16')
-    if not q.is_cuda or k_cache.device != device:
+    if index < 0:
         raise ValueError('q and the cache must be on the same CUDA device')
     strides = q.stride()
     if batch and strides[2] != 1:
         raise ValueError('q must have contiguous head elements')
-    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype)
+    cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index)
     kv_heads = k_cache.shape[1]
     if dim != k_cache.shape[3] or heads == 0 or heads % kv_heads:
         raise ValueError('q must match the cache\'s head_dim and have a multiple of its heads')
-    if page_table.ndim != 2 or page_table.shape[0] != batch or page_table.dtype != torch.int32 or page_table.device != device:
+    table = page_table.shape
+    if len(table) != 2 or table[0] != batch or page_table.dtype != torch.int32 or page_table.get_device() != index:
         raise ValueError('page_table must be int32 [batch, columns] on the cache\'s device')
     table_stride, step = page_table.stride()
-    columns = page_table.shape[1]
-    if columns > 1 and step != 1:
+    if step != 1 and table[1] > 1:
         raise ValueError('page_table must have contiguous rows')
-    _check_vector(lengths, 'lengths', torch.int32, batch, device)
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
+    _check_vector(lengths, 'lengths', torch.int32, batch, index)
+    if scale is None:
+        scale = dim ** -0.5
+    elif not math.isfinite(scale):
         raise ValueError('scale must be finite')
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.requires_grad and torch.is_grad_enabled():
         raise ValueError('inference only; use torch.inference_mode()')
     out = _output(q)
-    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+    lse = q.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
     if batch:
         if workspace is None:
-            workspace = N.workspace(device, paged_attention_workspace_bytes(1, heads, kv_heads, dim),
-                                    torch._C._cuda_getCurrentRawStream(device.index))
-        elif workspace.device != device or not workspace.is_contiguous():
+            workspace = N.workspace(q.device, paged_attention_workspace_bytes(1, heads, kv_heads, dim), _raw_stream(index))
+        elif workspace.get_device() != index or not workspace.is_contiguous():
             raise ValueError('workspace must be contiguous, on the cache\'s device')
-        _call(device, N.lib().kl_paged_attention, q.data_ptr(), strides[0], strides[1], _CODES[dtype], batch, heads, cache,
-              page_table.data_ptr(), table_stride, columns, lengths.data_ptr(), scale, out.data_ptr(),
+        _call(index, N.lib().kl_paged_attention, q.data_ptr(), strides[0], strides[1], _CODES[dtype], batch, heads, cache,
+              page_table.data_ptr(), table_stride, table[1], lengths.data_ptr(), scale, out.data_ptr(),
               None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.nbytes)
     return (out, lse) if return_lse else out
