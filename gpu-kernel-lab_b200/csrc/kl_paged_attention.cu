@@ -44,9 +44,10 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 2;
 constexpr int kMaxCtas = 640;          // bound of the grid: 3 per SM of up to 213 SMs
-constexpr int kMaxPrefetch = 16384;    // 128-byte lines
 constexpr int kRecordBytes = 16 * 1024;
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinBlocks = 3;         // per SM
+constexpr int join_heads(int hb) { return hb == 16 ? 4 : 2; }   // heads of one block of the join
 constexpr int kWholeUnits = 4;         // rows of up to so many units are not split
 constexpr int kMaxLens = 512;          // lengths kept in shared memory
 constexpr float kSlack = 8.0f;           // log2 of how far weights may exceed 1
@@ -228,9 +229,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   const int t4 = lane & 3, l4 = lane >> 2;
   const int rows = a.kv.kv_heads * a.blocks;        // rows per sequence
 
-  pdl_launch_dependents();                          // the join's blocks wait for this grid's end by themselves
-
-  // ---- what the first unit will wait for is brought into L2 while the lengths are read
+  // what the first units will wait for is brought into L2
   if (tid == 0) {
     prefetch_tmap(&maps.k);
     prefetch_tmap(&maps.v);
@@ -239,16 +238,9 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
       prefetch_tmap(&maps.vs);
     }
   }
-  {
-    const int row_lines = (a.columns + 31) / 32, head_lines = D * 2 / 128;
-    const long long table_lines = static_cast<long long>(a.batch) * row_lines, q_lines = static_cast<long long>(a.batch) * a.heads * head_lines;
-    for (int i = blockIdx.x * kThreads + tid; i < min(table_lines, static_cast<long long>(kMaxPrefetch)); i += gridDim.x * kThreads)
-      prefetch_l2(a.table + i / row_lines * a.table_stride + i % row_lines * 32);
-    for (int i = blockIdx.x * kThreads + tid; i < min(q_lines, static_cast<long long>(kMaxPrefetch)); i += gridDim.x * kThreads) {
-      const int h = i / head_lines;
-      prefetch_l2(static_cast<const char*>(a.q) + (h / a.heads * a.q_row_stride + h % a.heads * a.q_head_stride) * 2 + i % head_lines * 128);
-    }
-  }
+  if (blockIdx.x < a.batch && tid * 32 < a.columns) prefetch_l2(a.table + blockIdx.x * a.table_stride + tid * 32);
+  if (blockIdx.x < a.batch && tid < a.heads * (D / 64))
+    prefetch_l2(static_cast<const char*>(a.q) + (blockIdx.x * a.q_row_stride + tid / (D / 64) * a.q_head_stride) * 2 + tid % (D / 64) * 128);
 
   // ---- this CTA's units: one scan over the sequences' unit counts
   const long long room = static_cast<long long>(a.columns) * a.kv.page_size;
@@ -306,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
 #pragma unroll
   for (int end = 0; end < 2; ++end) {
     const int u = end ? hi : lo;
-    if ((incl - mine) * rows <= u && u < incl * rows) {
+    if ((end == 0 || !a.records) && (incl - mine) * rows <= u && u < incl * rows) {
       int before = (incl - mine) * rows, b = b0;
       for (;; ++b) {
         const int n = units_of(length_of(b)) * rows;
@@ -338,9 +330,13 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   Cursor in;                                        // next unit to fetch
   in.b = s_misc[8];
   load_len(in);
-  in.i = s_misc[9] % in.units;
-  in.head = s_misc[9] / in.units / a.blocks;
-  in.block = s_misc[9] / in.units % a.blocks;
+  in.head = s_misc[9] / in.units;
+  in.i = s_misc[9] - in.head * in.units;
+  in.block = 0;
+  if (a.blocks > 1) {
+    in.block = in.head % a.blocks;
+    in.head /= a.blocks;
+  }
   if (!a.records) {                                 // whole rows: those that begin in [lo, hi)
     if (hi < total) {
       const int units = units_of(s_misc[10] < kMaxLens ? s_len[s_misc[10]] : length_of(s_misc[10])), over = s_misc[11] % units;
@@ -761,13 +757,14 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
 
   // ---- main loop
   look_up();
+  start_row();
   fetch(0);
   if (count > 1) {
     advance(in);
     look_up();
   }
   int slot = 0;
-  bool fresh = true;
+  bool fresh = false;
   for (int u = 0; u < count; ++u, slot ^= 1) {
     if (u + 1 < count && !__any_sync(0xFFFFFFFFu, dead)) {
       fetch(slot ^ 1);
@@ -790,67 +787,72 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   if (tid == 0 && a.records) a.records[cta] = *s_piece;
 }
 
-// The rows that several CTAs have parts of: block (c, y) joins four heads of the row whose
-// first part is CTA c's. Launched behind the attention kernel as its programmatic dependent.
-// One block that joined a row inside that kernel, after an atomic arrival of each part, took
-// 8 us where this takes 3: a chain of round trips with the row's data going through one SM.
+// The rows that several CTAs have parts of: block (x, y) joins kHeads heads, from y * kHeads, of
+// the rows whose first part is CTA x's, x + gridDim.x's, and so on. Launched behind the
+// attention kernel as its programmatic dependent, so that the launch is under way when that
+// ends. Joining a row inside that kernel, in the CTA whose part arrives last, took
+// 8 us where this takes 4: a chain of round trips with the row's data going through one SM.
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Piece* records, const float* partials, T* out, float* lse) {
+__global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) join_kernel(const Piece* records, int count, const float* partials, T* out, float* lse) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kHeads = HB < 4 ? HB : 4, kVecs = kHeads * D / 4, kSides = kJoinThreads / kVecs;
+  constexpr int kHeads = join_heads(HB), kVecs = kHeads * D / 4, kSides = kJoinThreads / kVecs, kBatch = 8;
   __shared__ float4 s_v[kSides][kVecs];
   __shared__ float s_m[kSides][kVecs], s_l[kSides][kVecs];
   pdl_wait();
-  const Piece piece = records[blockIdx.x];
   const int side = threadIdx.x / kVecs, vec = threadIdx.x % kVecs;
   const int col = blockIdx.y * kHeads + vec / (D / 4), d = vec % (D / 4) * 4;
-  if (piece.ways == 0 || blockIdx.y * kHeads >= piece.heads) return;
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float m = -FLT_MAX, l = 0.0f;
-  if (col < piece.heads) {
-    for (int k0 = side; k0 < piece.ways; k0 += 8 * kSides) {
-      float4 y[8];
-      float pm[8], pl[8];
+  for (int c = blockIdx.x; c < count; c += gridDim.x) {
+    const Piece piece = records[c];
+    if (piece.ways == 0 || blockIdx.y * kHeads >= piece.heads) continue;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float m = -FLT_MAX, l = 0.0f;
+    if (col < piece.heads) {
+      for (int k0 = side; k0 < piece.ways; k0 += kBatch * kSides) {
+        float4 y[kBatch];
+        float pm[kBatch], pl[kBatch];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int k = k0 + i * kSides;
-        y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), pm[i] = -FLT_MAX, pl[i] = 0.0f;
-        if (k < piece.ways) {
-          const float* x = partials + static_cast<long long>((blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * (HB * (D + 2));
-          y[i] = __ldcg(reinterpret_cast<const float4*>(x + col * D + d));
-          pm[i] = __ldcg(x + HB * D + col);
-          pl[i] = __ldcg(x + HB * D + HB + col);
+        for (int i = 0; i < kBatch; ++i) {
+          const int k = k0 + i * kSides;
+          y[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), pm[i] = -FLT_MAX, pl[i] = 0.0f;
+          if (k < piece.ways) {
+            const float* x = partials + static_cast<long long>((c + k) * 2 + (k == 0 ? 1 : 0)) * (HB * (D + 2));
+            y[i] = __ldcg(reinterpret_cast<const float4*>(x + col * D + d));
+            pm[i] = __ldcg(x + HB * D + col);
+            pl[i] = __ldcg(x + HB * D + HB + col);
+          }
+        }
+        float most = m;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) most = fmaxf(most, pm[i]);
+        const float keep = ex2(m - most);
+        v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep, l *= keep;
+        m = most;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const float f = ex2(pm[i] - m);
+          v.x += f * y[i].x, v.y += f * y[i].y, v.z += f * y[i].z, v.w += f * y[i].w;
+          l += f * pl[i];
         }
       }
-      float most = m;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, pm[i]);
-      const float keep = ex2(m - most);
-      v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep, l *= keep;
-      m = most;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = ex2(pm[i] - m);
-        v.x += f * y[i].x, v.y += f * y[i].y, v.z += f * y[i].z, v.w += f * y[i].w;
-        l += f * pl[i];
-      }
     }
+    s_v[side][vec] = v;
+    s_m[side][vec] = m;
+    s_l[side][vec] = l;
+    __syncthreads();
+    if (side == 0 && col < piece.heads) {
+      for (int k = 1; k < kSides; ++k) m = fmaxf(m, s_m[k][vec]);
+      v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      l = 0.0f;
+      for (int k = 0; k < kSides; ++k) {
+        const float f = ex2(s_m[k][vec] - m);
+        const float4 y = s_v[k][vec];
+        v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
+        l += f * s_l[k][vec];
+      }
+      emit<kBf16, D>(out, lse, piece.row + col, d, v, m, l);
+    }
+    __syncthreads();
   }
-  s_v[side][vec] = v;
-  s_m[side][vec] = m;
-  s_l[side][vec] = l;
-  __syncthreads();
-  if (side > 0 || col >= piece.heads) return;
-  for (int k = 1; k < kSides; ++k) m = fmaxf(m, s_m[k][vec]);
-  v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  l = 0.0f;
-  for (int k = 0; k < kSides; ++k) {
-    const float f = ex2(s_m[k][vec] - m);
-    const float4 y = s_v[k][vec];
-    v.x += f * y.x, v.y += f * y.y, v.z += f * y.z, v.w += f * y.w;
-    l += f * s_l[k][vec];
-  }
-  emit<kBf16, D>(out, lse, piece.row + col, d, v, m, l);
 }
 
 // Tensor maps of K and V with boxes of as many rows as divide a page, at most `keys`;
@@ -916,7 +918,7 @@ cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   attn_kernel<T, INT8, D, HB><<<grid, kThreads, G::kSmem, s>>>(a, maps);
   if ((e = cudaGetLastError()) != cudaSuccess || !a.records) return e;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(grid, (std::min(a.group, HB) + 3) / 4);
+  config.gridDim = dim3(std::min<unsigned>(grid, kJoinBlocks * sm_count), (std::min(a.group, HB) + join_heads(HB) - 1) / join_heads(HB));
   config.blockDim = dim3(kJoinThreads);
   config.stream = s;
   cudaLaunchAttribute attr = {};
@@ -924,7 +926,7 @@ cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, join_kernel<T, D, HB>, static_cast<const Piece*>(a.records), static_cast<const float*>(a.partials),
+  return cudaLaunchKernelEx(&config, join_kernel<T, D, HB>, static_cast<const Piece*>(a.records), static_cast<int>(grid), static_cast<const float*>(a.partials),
                             static_cast<T*>(a.out), a.lse);
 }
 
