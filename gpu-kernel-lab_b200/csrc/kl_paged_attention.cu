@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     }
   };
   uint32_t armed = 0, phases = 0;                   // per slot: copies under way, parity of its barrier
-  bool holey = false;
+  uint32_t holey = 0;                               // per slot: some of its keys' pages were out of range
   const int group_gap = a.box == 16 ? 32 : 16;      // floats from the scales of 16 keys to the next: a box starts at 128 bytes
   auto fetch = [&](int slot) {
     const int count = in.len - (in.i * G::kUnit + warp * G::kKeys);
@@ -388,8 +388,9 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
       used[w] = row < G::kKeys && row < count;
       if (used[w] && static_cast<unsigned>(page[w]) >= static_cast<unsigned>(a.kv.pages)) used[w] = false, bad = true;
     }
-    holey |= __any_sync(0xFFFFFFFFu, bad);
-    if (holey) {                                    // some page id was out of range: its keys count as absent
+    holey &= ~(1u << slot);
+    if (__any_sync(0xFFFFFFFFu, bad)) {             // such keys count as absent
+      holey |= 1u << slot;
       if (bad) record_error(a.status, KL_ERR_INVALID);
 #pragma unroll
       for (int w = 0; w < kWords; ++w) {
@@ -506,12 +507,12 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     }
     __syncwarp();
     const int count = at.len - (at.i * G::kUnit + warp * G::kKeys);
-    const bool partial = count < G::kKeys || holey;
+    const bool holes = holey >> slot & 1, partial = count < G::kKeys || holes;
     unsigned valid[kWords];
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
       valid[w] = count >= 32 * w + 32 ? 0xFFFFFFFFu : count <= 32 * w ? 0u : (1u << (count - 32 * w)) - 1;
-      if (holey) valid[w] &= reinterpret_cast<const unsigned*>(note + slot * G::kNote + G::kNote - 128)[w];
+      if (holes) valid[w] &= reinterpret_cast<const unsigned*>(note + slot * G::kNote + G::kNote - 128)[w];
     }
     if (!INT8 && partial && a.box) {                // a box brings what the page holds past the length: values become 0
       for (int i = lane; i < G::kKeys * G::kRow / 16; i += 32) {
@@ -756,23 +757,22 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   };
 
   // ---- main loop
+  int fetched = 0;
+  auto fetch_next = [&](int slot) {
+    fetch(slot);
+    if (++fetched < count) {
+      advance(in);
+      look_up();
+    }
+  };
   look_up();
   start_row();
-  fetch(0);
-  if (count > 1) {
-    advance(in);
-    look_up();
-  }
-  int slot = 0;
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1 && i < count; ++i) fetch_next(i);
+  int slot = 0, fill = kStages - 1;
   bool fresh = false;
-  for (int u = 0; u < count; ++u, slot ^= 1) {
-    if (u + 1 < count && !__any_sync(0xFFFFFFFFu, dead)) {
-      fetch(slot ^ 1);
-      if (u + 2 < count) {
-        advance(in);
-        look_up();
-      }
-    }
+  for (int u = 0; u < count; ++u) {
+    if (fetched < count && !__any_sync(0xFFFFFFFFu, dead)) fetch_next(fill);
     if (fresh) start_row();
     compute(slot);
     fresh = at.i + 1 == at.units || u + 1 == count;
@@ -782,8 +782,9 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
       __syncthreads();
     }
     if (u + 1 < count) advance(at);
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+    fill = fill + 1 == kStages ? 0 : fill + 1;
   }
-
   if (tid == 0 && a.records) a.records[cta] = *s_piece;
 }
 

@@ -267,6 +267,25 @@ def test_attention_out_of_range_table_is_recorded_not_read():
     assert N.device_status(0, reset=True) == N.KL_OK
 
 
+@gpu
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("page", [16, 24])
+def test_attention_bad_pages_of_a_long_row_are_absent(quantized, page):
+    """Pages out of range here and there: as if the sequence consisted of the other pages."""
+    q, cache, table, _ = batch(generator(page), torch.bfloat16, quantized, 4, 2, 128, page, [page * 90, page * 7], poison=False)
+    lengths = torch.tensor([page * 90, page * 7], dtype=torch.int32, device="cuda")
+    gone = [3, 20, 21, 22, 23, 24, 25, 26, 27, 28, 50, 89]
+    bad = table.clone()
+    bad[0, gone] = torch.tensor([-1, 2 ** 30, cache.k_cache.shape[0]] * 4, dtype=torch.int32, device="cuda")
+    out = kl.paged_attention(q, cache.k_cache, cache.v_cache, bad, lengths, cache.k_scales, cache.v_scales)
+    assert N.device_status(0, reset=True) == N.KL_ERR_INVALID
+    kept = [i for i in range(90) if i not in gone]
+    short = table[:, :len(kept)].clone()
+    short[0] = table[0, kept]
+    ref, _, extra, _ = attention(q, cache, short, torch.tensor([page * len(kept), page * 7], dtype=torch.int32, device="cuda"))
+    close(out, ref, torch.bfloat16, extra)
+
+
 # ---- write and read -----------------------------------------------------------------
 def rope_tables(g, dim, positions=5000):
     turn = torch.arange(positions, device="cuda", dtype=torch.float64)[:, None] * 1e6 ** (
