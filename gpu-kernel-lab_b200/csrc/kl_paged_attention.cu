@@ -83,9 +83,12 @@ struct AttnArgs {
   int* status;
 };
 
-struct alignas(64) AttnMaps {
+template <bool INT8> struct alignas(64) AttnMaps {
   CUtensorMap k, v;                    // [page, head, token, element]
-  CUtensorMap ks, vs;                  // [page, head, token], int8 only
+};
+template <> struct alignas(64) AttnMaps<true> {
+  CUtensorMap k, v;
+  CUtensorMap ks, vs;                  // [page, head, token]
 };
 
 KL_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -207,7 +210,7 @@ KL_DEVICE void emit(T* out, float* lse, int row, int d, float4 v, float m, float
 
 template <typename T, bool INT8, int D, int HB>
 __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
-    attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps maps) {
+    attn_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ AttnMaps<INT8> maps) {
   using G = Geo<INT8, D, HB>;
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr bool kQkBf16 = kBf16;                   // type of the K Q^T product
@@ -860,8 +863,9 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) join_kernel(const P
 // returns the rows of a box, or 0 where the lanes have to copy: pages that are no
 // multiple of 8 tokens (a box of fewer rows would split a swizzle pattern) or, in int8,
 // of 16 (the unit in which the scales are laid out), and scales that TMA cannot take.
-int make_maps(const AttnArgs& a, AttnMaps& maps, int head_dim, int elem, int span, int keys) {
-  const int least = elem == 1 ? 16 : 8;
+template <bool INT8>
+int make_maps(const AttnArgs& a, AttnMaps<INT8>& maps, int head_dim, int span, int keys) {
+  const int elem = INT8 ? 1 : 2, least = INT8 ? 16 : 8;
   int box = keys;
   while (box >= least && a.kv.page_size % box) box /= 2;
   if (box < least) return 0;
@@ -880,7 +884,7 @@ int make_maps(const AttnArgs& a, AttnMaps& maps, int head_dim, int elem, int spa
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return 0;
   }
-  if (elem == 1) {
+  if constexpr (INT8) {
     if (a.kv.s_token_stride != 1) return 0;
     const cuuint64_t s_strides[2] = {static_cast<cuuint64_t>(a.kv.s_head_stride * 4), static_cast<cuuint64_t>(a.kv.s_page_stride * 4)};
     const cuuint32_t s_tile[3] = {static_cast<cuuint32_t>(box), 1, 1};
@@ -897,8 +901,8 @@ int make_maps(const AttnArgs& a, AttnMaps& maps, int head_dim, int elem, int spa
 template <typename T, bool INT8, int D, int HB>
 cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   using G = Geo<INT8, D, HB>;
-  AttnMaps maps;
-  a.box = make_maps(a, maps, D, G::kElem, G::kSpan, G::kKeys);
+  AttnMaps<INT8> maps;
+  a.box = make_maps(a, maps, D, G::kSpan, G::kKeys);
   // once per device: allow the shared memory
   static std::atomic<unsigned long long> allowed{0};
   int dev = 0;
