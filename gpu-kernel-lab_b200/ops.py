@@ -18,6 +18,8 @@ int8 ``[N, K]``, packed nibbles uint8 ``[N, K/2]`` or bf16 ``[N, K]``):
   -> (values, ids)`` -- the fused lm_head top-k (no logits are written)
 * ``project(x, w, scales, inverse, group, warps, persistent, swiglu) -> y`` --
   the reference op's signature (``warp_gemv.cu:56-58``)
+* ``paged_attention``, ``qk_norm_rope_write`` (which mutates the cache) and ``read_kv`` -- the
+  operators of ``paged_kv.py``, whose functions call them where they are traced
 * ``int4_gemv(x, data, scales, group, block_n) -> y`` and
   ``int4_lm_head_topk(x, data, scales, group, top_k, block_n) -> (values, ids)``
   (``learning/09_int4/kernels.py:67-99``)
@@ -189,4 +191,54 @@ def _int4_head_fake(x, data, scales, group, top_k, block_n):
     return x.new_empty(top_k, dtype=torch.float32), x.new_empty(top_k, dtype=torch.int64)
 
 
-OPS = ("linear", "linear_out", "linear_topk", "project", "int4_gemv", "int4_lm_head_topk")
+# ---- paged key-value cache ----------------------------------------------------------
+_lib.define("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor lengths, "
+            "Tensor? k_scales=None, Tensor? v_scales=None, float? scale=None) -> (Tensor, Tensor)")
+_lib.define("qk_norm_rope_write(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, "
+            "Tensor positions, Tensor slots, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scales=None, "
+            "Tensor(d!)? v_scales=None, float epsilon=1e-6) -> Tensor")
+_lib.define("read_kv(Tensor k_cache, Tensor v_cache, Tensor slots, Tensor? k_scales=None, Tensor? v_scales=None, "
+            "ScalarType? dtype=None) -> (Tensor, Tensor)")
+
+
+def _paged_attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None):
+    from . import paged_kv
+    return paged_kv.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, return_lse=True)
+
+
+def _qk_norm_rope_write_cuda(*args, **kwargs):
+    from . import paged_kv
+    return paged_kv.qk_norm_rope_write(*args, **kwargs)
+
+
+def _read_kv_cuda(*args, **kwargs):
+    from . import paged_kv
+    return paged_kv.read_kv(*args, **kwargs)
+
+
+_lib.impl("paged_attention", _paged_attention_cuda, "CUDA")
+_lib.impl("qk_norm_rope_write", _qk_norm_rope_write_cuda, "CUDA")
+_lib.impl("read_kv", _read_kv_cuda, "CUDA")
+
+
+@torch.library.register_fake("kl_b200::paged_attention")
+def _paged_attention_fake(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@torch.library.register_fake("kl_b200::qk_norm_rope_write")
+def _qk_norm_rope_write_fake(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales=None,
+                             v_scales=None, epsilon=1e-6):
+    return q.new_empty(q.shape)
+
+
+@torch.library.register_fake("kl_b200::read_kv")
+def _read_kv_fake(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
+    if dtype is None:
+        dtype = torch.bfloat16 if k_cache.dtype == torch.int8 else k_cache.dtype
+    shape = (slots.numel(), k_cache.shape[1], k_cache.shape[3])
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
+OPS = ("linear", "linear_out", "linear_topk", "project", "int4_gemv", "int4_lm_head_topk", "paged_attention",
+       "qk_norm_rope_write", "read_kv")

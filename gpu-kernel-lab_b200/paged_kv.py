@@ -23,7 +23,8 @@ Arguments are checked on the host (``ValueError``).  What only the device sees
 outside the buffers and is recorded for ``_native.device_status``.
 
 The functions are for inference: tensors that require grad are refused, as
-``qwen_rmsnorm`` refuses them.
+``qwen_rmsnorm`` refuses them.  Called eagerly they launch directly; where torch
+traces them they are the operators ``torch.ops.kl_b200.*`` of the same names.
 """
 from __future__ import annotations
 
@@ -148,6 +149,9 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
 
     The arithmetic is f32 up to one rounding at the store (an int8 cache quantises the f32 value).
     """
+    if torch.compiler.is_compiling():
+        return torch.ops.kl_b200.qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache,
+                                                    k_scales, v_scales, epsilon)
     shape, kv_shape = q.shape, k.shape
     if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape or shape[0] != kv_shape[0] or shape[2] != kv_shape[2]:
         raise ValueError('q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]')
@@ -195,6 +199,8 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
 
     ``dtype`` (bf16 or f16) is that of the result of an int8 cache, bf16 if not given; a 16-bit cache returns its own.
     """
+    if torch.compiler.is_compiling():
+        return torch.ops.kl_b200.read_kv(k_cache, v_cache, slots, k_scales, v_scales, dtype)
     if dtype is None:
         dtype = torch.bfloat16 if k_cache.dtype == torch.int8 else k_cache.dtype
     if dtype not in _CODES:
@@ -224,6 +230,9 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     exponentials (``-inf`` for a length of 0), by which parts of a sequence can be joined.  ``workspace`` (uint8, zeroed
     once, of ``paged_attention_workspace_bytes``) takes the place of the scratch kept per device and stream.
     """
+    if torch.compiler.is_compiling():
+        both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale)
+        return both if return_lse else both[0]
     shape = q.shape
     if len(shape) != 3:
         raise ValueError('q must be [batch, heads, head_dim]')

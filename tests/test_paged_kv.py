@@ -564,3 +564,55 @@ def test_kv_slots():
     table = torch.tensor([[4, 2], [0, 9]], dtype=torch.int32)
     rows, positions = torch.tensor([0, 0, 1]), torch.tensor([3, 17, 16])
     assert kl.kv_slots(table, rows, positions, 16).tolist() == [67, 33, 144]
+
+
+# ---- as operators of torch, and together ------------------------------------------------
+def test_registered_operators_and_fake_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    schema = torch.ops.kl_b200.qk_norm_rope_write.default._schema
+    assert [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write] == [
+        "k_cache", "v_cache", "k_scales", "v_scales"]
+    with FakeTensorMode():
+        q, k = (torch.empty(5, h, 128, dtype=torch.bfloat16, device="cuda") for h in (4, 2))
+        cache = torch.empty(3, 2, 16, 128, dtype=torch.bfloat16, device="cuda")
+        at, cos = torch.empty(5, dtype=torch.int64, device="cuda"), torch.empty(9, 64, device="cuda")
+        out = torch.ops.kl_b200.qk_norm_rope_write(q, k, k, None, None, cos, cos, at, at, cache, cache)
+        assert out.shape == q.shape and out.dtype == torch.bfloat16
+        o, lse = torch.ops.kl_b200.paged_attention(q, cache, cache, torch.empty(5, 3, dtype=torch.int32, device="cuda"), at.int())
+        assert o.shape == q.shape and lse.shape == (5, 4) and lse.dtype == torch.float32
+        a, b = torch.ops.kl_b200.read_kv(cache.to(torch.int8), cache.to(torch.int8), at, dtype=torch.float16)
+        assert a.shape == b.shape == (5, 2, 128) and a.dtype == torch.float16
+
+
+@gpu
+def test_compiled_calls_equal_eager_ones():
+    q, cache, table, lengths = batch(generator(14), torch.bfloat16, True, 4, 2, 64, 16, [100, 7], poison=False)
+    k = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    cos, sin = rope_tables(None, 64, 200)
+    positions = lengths.long() - 1
+    slots = kl.kv_slots(table, torch.arange(2, device="cuda"), positions, 16)
+
+    def step(q, k, v, c, d, cs, ds):
+        q = kl.qk_norm_rope_write(q, k, v, None, None, cos, sin, positions, slots, c, d, cs, ds)
+        out, lse = kl.paged_attention(q, c, d, table, lengths, cs, ds, return_lse=True)
+        return out * 2, lse, *kl.read_kv(c, d, slots, cs, ds)
+
+    mine, other = ([t.clone() for t in cache] for _ in range(2))
+    eager = step(q, k, k, *mine)
+    compiled = torch.compile(step, backend="aot_eager", fullgraph=True)(q, k, k, *other)
+    assert all(torch.equal(a, b) for a, b in zip(eager, compiled))
+    assert all(torch.equal(a, b) for a, b in zip(mine, other))
+
+
+@gpu
+@pytest.mark.parametrize("int8_cache", [False, True])
+def test_example_decodes_like_the_uncached_sequence(int8_cache):
+    import importlib.util
+    from tests.conftest import ROOT
+    spec = importlib.util.spec_from_file_location("paged_decode", ROOT / "examples" / "paged_decode.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    error, _ = example.main(batch=3, prompt=77, steps=5, int8_cache=int8_cache)
+    # bf16 attention outputs differ by up to two roundings (2^-7); int8 keys and values by a step's half of their largest element,
+    # 1/254 of about three times their root mean square, averaged over the sequence
+    assert error < (2.0 ** -7 + 3 / 254 if int8_cache else 2.0 ** -7)
