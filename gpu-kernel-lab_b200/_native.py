@@ -44,6 +44,10 @@ class KlProblem(ctypes.Structure):
 
 #: ``kl_kv_cache`` of include/kl_b200.h, packed into bytes: four pointers, six strides, five ints
 KV_CACHE = struct.Struct("@4P6q5i4x")
+#: ``kl_kv_write_args`` and ``kl_paged_attention_args``, the packed cache in their middle (one packed argument takes ctypes
+#: a third of the time of twenty)
+KV_WRITE_ARGS = struct.Struct("@10P6q104s4if4x")
+PAGED_ATTENTION_ARGS = struct.Struct("@6PN3q104s4if4x")
 
 _P, _I, _S, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_longlong
 _SIGNATURES = {
@@ -74,10 +78,9 @@ _SIGNATURES = {
     "kl_rmsnorm": (_I, [_P, _P, _P, _I, _I, _I, ctypes.c_float, _I, _P, _P, _P]),
     "kl_linear_topk": (_I, [_P, _I, _I, _I, _P, _I, _I, _I, _P, _P, _I, ctypes.c_longlong, _P, _P, _P, _S, _I, _P]),
     "kl_linear_topk_workspace_bytes": (_S, [_I, _I, _I, _I, _I]),
-    "kl_qk_norm_rope_write": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P,
-                                   ctypes.c_float, _P, _P, _P]),
+    "kl_qk_norm_rope_write": (_I, [_P, _P]),
     "kl_read_kv": (_I, [_P, _I, _P, _I, _P, _P, _P]),
-    "kl_paged_attention": (_I, [_P, _L, _L, _I, _I, _I, _P, _P, _L, _I, _P, ctypes.c_float, _P, _P, _P, _S, _P]),
+    "kl_paged_attention": (_I, [_P, _P]),
     "kl_paged_attention_workspace_bytes": (_S, [_I, _I, _I, _I]),
 }
 

@@ -914,29 +914,24 @@ int validate_cache(const kl_kv_cache* c, int dtype) {
 
 }  // namespace
 
-int kl_qk_norm_rope_write(const void* q, long long q_token_stride, long long q_head_stride, const void* k,
-                          long long k_token_stride, long long k_head_stride, const void* v, long long v_token_stride,
-                          long long v_head_stride, int dtype, int tokens, int heads, const void* q_weight,
-                          const void* k_weight, const float* cos, const float* sin, int max_positions,
-                          const int64_t* positions, const int64_t* slots, float eps, const kl_kv_cache* cache, void* q_out,
-                          void* stream) {
-  int rc = validate_cache(cache, dtype);
+int kl_qk_norm_rope_write(const kl_kv_write_args* args, void* stream) {
+  if (!args) return fail(KL_ERR_INVALID, "args must be non-null");
+  const kl_kv_write_args& a = *args;
+  int rc = validate_cache(&a.cache, a.dtype);
   if (rc != KL_OK) return rc;
-  if (tokens < 0 || heads <= 0) return fail(KL_ERR_INVALID, "need tokens >= 0 and heads > 0");
-  if ((q_weight == nullptr) != (k_weight == nullptr))
+  if (a.tokens < 0 || a.heads <= 0) return fail(KL_ERR_INVALID, "need tokens >= 0 and heads > 0");
+  if ((a.q_weight == nullptr) != (a.k_weight == nullptr))
     return fail(KL_ERR_INVALID, "q_weight and k_weight must be given together");
-  if (q_weight && (!(eps > 0.0f) || !(eps < 3.0e38f))) return fail(KL_ERR_INVALID, "epsilon must be finite and positive");
-  if (max_positions <= 0) return fail(KL_ERR_INVALID, "the rotary table is empty");
-  if (tokens == 0) return KL_OK;
-  if (!q || !k || !v || !cos || !sin || !positions || !slots || !q_out)
+  if (a.q_weight && (!(a.eps > 0.0f) || !(a.eps < 3.0e38f))) return fail(KL_ERR_INVALID, "epsilon must be finite and positive");
+  if (a.max_positions <= 0) return fail(KL_ERR_INVALID, "the rotary table is empty");
+  if (a.tokens == 0) return KL_OK;
+  if (!a.q || !a.k || !a.v || !a.cos || !a.sin || !a.positions || !a.slots || !a.q_out)
     return fail(KL_ERR_INVALID, "q, k, v, cos, sin, positions, slots and q_out must be non-null");
-  if (static_cast<long long>(tokens) * (heads + 2ll * cache->kv_heads) > 0x7FFFFFFFll)
+  if (static_cast<long long>(a.tokens) * (a.heads + 2ll * a.cache.kv_heads) > 0x7FFFFFFFll)
     return fail(KL_ERR_INVALID, "tokens * (heads + 2 kv_heads) must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
-  const KvRows x[3] = {{q, q_token_stride, q_head_stride}, {k, k_token_stride, k_head_stride}, {v, v_token_stride, v_head_stride}};
-  const cudaError_t e = launch_kv_write(x, dtype, tokens, heads, q_weight, k_weight, cos, sin, max_positions, positions, slots,
-                                        eps, *cache, q_out, di.sm_count, di.status, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_kv_write(a, di.sm_count, di.status, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "KV write launch");
 }
 
@@ -957,35 +952,35 @@ int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int to
 
 size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  return paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim, sm_count_or_default());
+  return paged_attention_workspace_bytes(heads, kv_heads, head_dim, sm_count_or_default());
 }
 
-int kl_paged_attention(const void* q, long long q_row_stride, long long q_head_stride, int dtype, int batch, int heads,
-                       const kl_kv_cache* cache, const int32_t* page_table, long long table_stride, int columns,
-                       const int32_t* lengths, float scale, void* out, float* lse, void* workspace, size_t workspace_bytes,
-                       void* stream) {
-  int rc = validate_cache(cache, dtype);
+int kl_paged_attention(const kl_paged_attention_args* args, void* stream) {
+  if (!args) return fail(KL_ERR_INVALID, "args must be non-null");
+  const kl_paged_attention_args& a = *args;
+  const kl_kv_cache& c = a.cache;
+  int rc = validate_cache(&c, a.dtype);
   if (rc != KL_OK) return rc;
-  if (batch < 0 || heads <= 0 || columns < 0 || heads % cache->kv_heads)
+  if (a.batch < 0 || a.heads <= 0 || a.columns < 0 || a.heads % c.kv_heads)
     return fail(KL_ERR_INVALID, "need batch >= 0, columns >= 0 and heads a multiple of kv_heads");
-  if (!(scale > -3.0e38f && scale < 3.0e38f)) return fail(KL_ERR_INVALID, "scale must be finite");
-  if (batch == 0) return KL_OK;
-  if (!q || !lengths || !out || (columns > 0 && !page_table)) return fail(KL_ERR_INVALID, "q, page_table, lengths and out must be non-null");
-  if (!aligned16(out)) return fail(KL_ERR_INVALID, "out must be 16-byte aligned");
-  if (static_cast<long long>(columns) * cache->page_size > 0x7FFF0000ll || static_cast<long long>(batch) * heads > 0x7FFFFFFFll)
+  if (!(a.scale > -3.0e38f && a.scale < 3.0e38f)) return fail(KL_ERR_INVALID, "scale must be finite");
+  if (a.batch == 0) return KL_OK;
+  if (!a.q || !a.lengths || !a.out || (a.columns > 0 && !a.page_table))
+    return fail(KL_ERR_INVALID, "q, page_table, lengths and out must be non-null");
+  if (!aligned16(a.out)) return fail(KL_ERR_INVALID, "out must be 16-byte aligned");
+  const long long room = static_cast<long long>(a.columns) * c.page_size;
+  if (room > 0x7FFF0000ll || static_cast<long long>(a.batch) * a.heads > 0x7FFFFFFFll)
     return fail(KL_ERR_INVALID, "columns * page_size and batch * heads must stay below 2^31");
   // units of at least 64 keys; the kernel counts them in 32 bits
-  if (static_cast<long long>(batch) * heads * ((static_cast<long long>(columns) * cache->page_size + 63) / 64) > 0x7FFFFFFFll)
+  if (static_cast<long long>(a.batch) * a.heads * ((room + 63) / 64) > 0x7FFFFFFFll)
     return fail(KL_ERR_INVALID, "batch * heads * columns * page_size / 64 must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
-  const size_t need = paged_attention_workspace_bytes(batch, heads, cache->kv_heads, cache->head_dim, di.sm_count);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(KL_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : 0);
-  if (!aligned16(workspace)) return fail(KL_ERR_INVALID, "workspace must be 16-byte aligned");
-  const cudaError_t e = launch_paged_attention(q, dtype, batch, heads, q_row_stride, q_head_stride, *cache, page_table, table_stride,
-                                               columns, lengths, scale, out, lse, workspace, di.sm_count, di.status,
-                                               static_cast<cudaStream_t>(stream));
+  const size_t need = paged_attention_workspace_bytes(a.heads, c.kv_heads, c.head_dim, di.sm_count);
+  if (!a.workspace || a.workspace_bytes < need)
+    return fail(KL_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, a.workspace ? a.workspace_bytes : 0);
+  if (!aligned16(a.workspace)) return fail(KL_ERR_INVALID, "workspace must be 16-byte aligned");
+  const cudaError_t e = launch_paged_attention(a, di.sm_count, di.status, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? KL_OK : cuda_fail(e, "paged attention launch");
 }
 

@@ -247,26 +247,15 @@ cudaError_t launch_topk_merge_rows(const int64_t* packed, int rows, int count, i
 // ------------------------------------------------- paged key-value cache
 struct KvView;
 KvView kv_view(const kl_kv_cache& c);
-// [tokens, heads, head_dim] rows with contiguous elements; strides in elements
-struct KvRows {
-  const void* data;
-  long long token_stride, head_stride;
-};
-// x: the rows of q, k and v; q_weight/k_weight both null without the norm (kl_kv.cu)
-cudaError_t launch_kv_write(const KvRows x[3], int dtype, int tokens, int heads, const void* q_weight, const void* k_weight,
-                            const float* cos, const float* sin, int max_positions, const int64_t* positions,
-                            const int64_t* slots, float eps, const kl_kv_cache& cache, void* q_out, int sm_count,
-                            int* status, cudaStream_t s);
+// kl_kv.cu
+cudaError_t launch_kv_write(const kl_kv_write_args& args, int sm_count, int* status, cudaStream_t s);
 cudaError_t launch_kv_read(const kl_kv_cache& cache, int dtype, const int64_t* slots, int tokens, void* k, void* v,
                            int sm_count, int* status, cudaStream_t s);
 // cuTensorMapEncodeTiled (PFN_cuTensorMapEncodeTiled_v12000), or null
 void* tensor_map_encoder();
 // kl_paged_attention.cu
-size_t paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int sm_count);
-cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int heads, long long q_row_stride,
-                                   long long q_head_stride, const kl_kv_cache& cache, const int* table, long long table_stride,
-                                   int columns, const int* lengths, float scale, void* out, float* lse, void* workspace,
-                                   int sm_count, int* status, cudaStream_t s);
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int sm_count);
+cudaError_t launch_paged_attention(const kl_paged_attention_args& args, int sm_count, int* status, cudaStream_t s);
 
 // ---------------------------------------------------------- quantisation
 cudaError_t launch_quantize_w8_row(const void* w, int w_dtype, int n, int k, int8_t* q, void* scale, cudaStream_t s);

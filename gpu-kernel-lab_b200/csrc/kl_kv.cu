@@ -504,7 +504,9 @@ cudaError_t read_d(const KvView& kv, int head_dim, const int64_t* slots, int tok
                            : read_t<T, INT8, 256>(kv, slots, tokens, k, v, status, sm_count, s);
 }
 
-KvView view_of(const kl_kv_cache& c) {
+}  // namespace
+
+KvView kv_view(const kl_kv_cache& c) {
   KvView v;
   v.k = static_cast<char*>(c.k);
   v.v = static_cast<char*>(c.v);
@@ -522,42 +524,37 @@ KvView view_of(const kl_kv_cache& c) {
   return v;
 }
 
-}  // namespace
-
-KvView kv_view(const kl_kv_cache& c) { return view_of(c); }
-
-cudaError_t launch_kv_write(const KvRows x[3], int dtype, int tokens, int heads, const void* q_weight, const void* k_weight,
-                            const float* cos, const float* sin, int max_positions, const int64_t* positions,
-                            const int64_t* slots, float eps, const kl_kv_cache& cache, void* q_out, int sm_count, int* status,
-                            cudaStream_t s) {
+cudaError_t launch_kv_write(const kl_kv_write_args& w, int sm_count, int* status, cudaStream_t s) {
   KvWriteArgs a;
-  for (int i = 0; i < 3; ++i) {
-    a.x[i] = static_cast<const char*>(x[i].data);
-    a.token_stride[i] = x[i].token_stride;
-    a.head_stride[i] = x[i].head_stride;
-  }
-  a.weight[0] = q_weight;
-  a.weight[1] = k_weight;
-  a.cos = cos;
-  a.sin = sin;
-  a.positions = positions;
-  a.slots = slots;
-  a.tokens = tokens;
-  a.heads = heads;
-  a.max_positions = max_positions;
-  a.eps = eps;
-  a.q_out = q_out;
-  a.kv = view_of(cache);
+  a.x[0] = static_cast<const char*>(w.q);
+  a.x[1] = static_cast<const char*>(w.k);
+  a.x[2] = static_cast<const char*>(w.v);
+  a.token_stride[0] = w.q_token_stride, a.head_stride[0] = w.q_head_stride;
+  a.token_stride[1] = w.k_token_stride, a.head_stride[1] = w.k_head_stride;
+  a.token_stride[2] = w.v_token_stride, a.head_stride[2] = w.v_head_stride;
+  a.weight[0] = w.q_weight;
+  a.weight[1] = w.k_weight;
+  a.cos = w.cos;
+  a.sin = w.sin;
+  a.positions = w.positions;
+  a.slots = w.slots;
+  a.tokens = w.tokens;
+  a.heads = w.heads;
+  a.max_positions = w.max_positions;
+  a.eps = w.eps;
+  a.q_out = w.q_out;
+  a.kv = kv_view(w.cache);
   a.status = status;
-  const bool int8 = cache.format == KL_KV_INT8;
-  if (dtype == KL_DT_BF16)
-    return int8 ? write_d<__nv_bfloat16, true>(a, cache.head_dim, sm_count, s) : write_d<__nv_bfloat16, false>(a, cache.head_dim, sm_count, s);
-  return int8 ? write_d<__half, true>(a, cache.head_dim, sm_count, s) : write_d<__half, false>(a, cache.head_dim, sm_count, s);
+  const bool int8 = w.cache.format == KL_KV_INT8;
+  const int dim = w.cache.head_dim;
+  if (w.dtype == KL_DT_BF16)
+    return int8 ? write_d<__nv_bfloat16, true>(a, dim, sm_count, s) : write_d<__nv_bfloat16, false>(a, dim, sm_count, s);
+  return int8 ? write_d<__half, true>(a, dim, sm_count, s) : write_d<__half, false>(a, dim, sm_count, s);
 }
 
 cudaError_t launch_kv_read(const kl_kv_cache& cache, int dtype, const int64_t* slots, int tokens, void* k, void* v,
                            int sm_count, int* status, cudaStream_t s) {
-  const KvView kv = view_of(cache);
+  const KvView kv = kv_view(cache);
   const bool int8 = cache.format == KL_KV_INT8;
   if (dtype == KL_DT_BF16)
     return int8 ? read_d<__nv_bfloat16, true>(kv, cache.head_dim, slots, tokens, k, v, status, sm_count, s)

@@ -955,46 +955,42 @@ cudaError_t attn_t(AttnArgs& a, int head_dim, int sm_count, cudaStream_t s) {
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim, int sm_count) {
-  // two partial rows per CTA of the widest wave
-  (void)batch;
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int sm_count) {
+  // the records, and two partial rows per CTA of the widest wave
   const int hb = heads_per_cta(heads / std::max(1, kv_heads), head_dim);
   return kCounterBytes + kRecordBytes + 2ull * std::min(3 * sm_count, kMaxCtas) * hb * (head_dim + 2) * sizeof(float);
 }
 
-cudaError_t launch_paged_attention(const void* q, int dtype, int batch, int heads, long long q_row_stride,
-                                   long long q_head_stride, const kl_kv_cache& cache, const int* table, long long table_stride,
-                                   int columns, const int* lengths, float scale, void* out, float* lse, void* workspace,
-                                   int sm_count, int* status, cudaStream_t s) {
+cudaError_t launch_paged_attention(const kl_paged_attention_args& p, int sm_count, int* status, cudaStream_t s) {
+  const int dim = p.cache.head_dim;
   AttnArgs a;
-  a.q = q;
-  a.q_row_stride = q_row_stride;
-  a.q_head_stride = q_head_stride;
-  a.kv = kv_view(cache);
-  a.table = table;
-  a.table_stride = table_stride;
-  a.lengths = lengths;
-  a.batch = batch;
-  a.heads = heads;
-  a.columns = columns;
-  a.group = heads / cache.kv_heads;
-  const int hb = heads_per_cta(a.group, cache.head_dim);
+  a.q = p.q;
+  a.q_row_stride = p.q_row_stride;
+  a.q_head_stride = p.q_head_stride;
+  a.kv = kv_view(p.cache);
+  a.table = p.page_table;
+  a.table_stride = p.table_stride;
+  a.lengths = p.lengths;
+  a.batch = p.batch;
+  a.heads = p.heads;
+  a.columns = p.columns;
+  a.group = p.heads / p.cache.kv_heads;
+  const int hb = heads_per_cta(a.group, dim);
   a.blocks = (a.group + hb - 1) / hb;
-  a.q_vec = (reinterpret_cast<uintptr_t>(q) % 4 == 0) && q_row_stride % 2 == 0 && q_head_stride % 2 == 0;
+  a.q_vec = (reinterpret_cast<uintptr_t>(p.q) % 4 == 0) && p.q_row_stride % 2 == 0 && p.q_head_stride % 2 == 0;
   int log = 0;
-  while ((1ll << log) < cache.page_size) ++log;
-  a.page_mul = static_cast<uint32_t>(((1ull << (31 + log)) + cache.page_size - 1) / cache.page_size);
+  while ((1ll << log) < p.cache.page_size) ++log;
+  a.page_mul = static_cast<uint32_t>(((1ull << (31 + log)) + p.cache.page_size - 1) / p.cache.page_size);
   a.page_shift = 31 + log;
-  a.scale = scale;
-  a.out = out;
-  a.lse = lse;
-  a.workspace = workspace;
+  a.scale = p.scale;
+  a.out = p.out;
+  a.lse = p.lse;
+  a.workspace = p.workspace;
   a.status = status;
-  const bool int8 = cache.format == KL_KV_INT8;
-  if (dtype == KL_DT_BF16)
-    return int8 ? attn_t<__nv_bfloat16, true>(a, cache.head_dim, sm_count, s)
-                : attn_t<__nv_bfloat16, false>(a, cache.head_dim, sm_count, s);
-  return int8 ? attn_t<__half, true>(a, cache.head_dim, sm_count, s) : attn_t<__half, false>(a, cache.head_dim, sm_count, s);
+  const bool int8 = p.cache.format == KL_KV_INT8;
+  if (p.dtype == KL_DT_BF16)
+    return int8 ? attn_t<__nv_bfloat16, true>(a, dim, sm_count, s) : attn_t<__nv_bfloat16, false>(a, dim, sm_count, s);
+  return int8 ? attn_t<__half, true>(a, dim, sm_count, s) : attn_t<__half, false>(a, dim, sm_count, s);
 }
 
 }  // namespace kl

@@ -167,7 +167,7 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
     cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index)
     if kv_shape[1] != k_cache.shape[1] or dim != k_cache.shape[3]:
         raise ValueError('k and v must match the cache\'s heads and head_dim')
-    q_weight_at = k_weight_at = None
+    q_weight_at = k_weight_at = 0
     if q_weight is not None and k_weight is not None:
         _check_vector(q_weight, 'q_weight', dtype, dim, index)
         _check_vector(k_weight, 'k_weight', dtype, dim, index)
@@ -188,9 +188,10 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
         raise ValueError('inference only; use torch.inference_mode()')
     out = _empty(q, (tokens, heads, dim), dtype, index)
     if tokens:
-        _call(index, N.lib().kl_qk_norm_rope_write, q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0],
-              sv[1], _CODES[dtype], tokens, heads, q_weight_at, k_weight_at, cos.data_ptr(), sin.data_ptr(), table[0],
-              positions.data_ptr(), slots.data_ptr(), epsilon, cache, out.data_ptr())
+        args = N.KV_WRITE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_weight_at, k_weight_at, cos.data_ptr(),
+                                    sin.data_ptr(), positions.data_ptr(), slots.data_ptr(), out.data_ptr(), sq[0], sq[1], sk[0],
+                                    sk[1], sv[0], sv[1], cache, _CODES[dtype], tokens, heads, table[0], epsilon)
+        _call(index, N.lib().kl_qk_norm_rope_write, args)
     return out
 
 
@@ -269,7 +270,9 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
             workspace = N.workspace(q.device, paged_attention_workspace_bytes(1, heads, kv_heads, dim), _raw_stream(index))
         elif workspace.get_device() != index or not workspace.is_contiguous():
             raise ValueError('workspace must be contiguous, on the cache\'s device')
-        _call(index, N.lib().kl_paged_attention, q.data_ptr(), strides[0], strides[1], _CODES[dtype], batch, heads, cache,
-              page_table.data_ptr(), table_stride, table[1], lengths.data_ptr(), scale, out.data_ptr(),
-              None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.nbytes)
+        args = N.PAGED_ATTENTION_ARGS.pack(
+            q.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            workspace.data_ptr(), workspace.nbytes, strides[0], strides[1], table_stride, cache, _CODES[dtype], batch, heads, table[1],
+            scale)
+        _call(index, N.lib().kl_paged_attention, args)
     return (out, lse) if return_lse else out

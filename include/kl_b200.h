@@ -327,15 +327,25 @@ typedef struct kl_kv_cache {
  *   otherwise distinct.  A position or slot out of range records
  *   KL_ERR_INVALID in the device status word; such a slot is not written and
  *   such a position is taken as 0.
- *   q_out [tokens, heads, head_dim] contiguous; it may be q only where q is
- *   contiguous too.
+ *   q_out [tokens, heads, head_dim] contiguous.
  */
-int kl_qk_norm_rope_write(const void* q, long long q_token_stride, long long q_head_stride,
-                          const void* k, long long k_token_stride, long long k_head_stride,
-                          const void* v, long long v_token_stride, long long v_head_stride,
-                          int dtype, int tokens, int heads, const void* q_weight, const void* k_weight,
-                          const float* cos, const float* sin, int max_positions, const int64_t* positions,
-                          const int64_t* slots, float eps, const kl_kv_cache* cache, void* q_out, void* stream);
+typedef struct kl_kv_write_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  const int64_t* slots;
+  void* q_out;
+  long long q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  kl_kv_cache cache;
+  int dtype, tokens, heads, max_positions;
+  float eps;
+} kl_kv_write_args;
+int kl_qk_norm_rope_write(const kl_kv_write_args* args, void* stream);
 
 /*
  * Keys and values of the given slots, dequantised: k and v [tokens, kv_heads,
@@ -360,15 +370,25 @@ int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int to
  *   past a sequence's length are not read.  A length beyond columns *
  *   page_size is cut to it, and keys of a page id out of range count
  *   as absent; both record KL_ERR_INVALID in the device status word.
- *   workspace: kl_paged_attention_workspace_bytes(...) bytes under kl_linear's
- *   workspace rule (its first 64 KiB zero before the first use; the calls leave
- *   it zero).
+ *   workspace: kl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned.
+ *   It may be kl_linear's: the first 64 KiB, which that needs zeroed, are left as
+ *   they are.  Calls that share a workspace must not run concurrently.
  */
 size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim);
-int kl_paged_attention(const void* q, long long q_row_stride, long long q_head_stride, int dtype, int batch, int heads,
-                       const kl_kv_cache* cache, const int32_t* page_table, long long table_stride, int columns,
-                       const int32_t* lengths, float scale, void* out, float* lse, void* workspace,
-                       size_t workspace_bytes, void* stream);
+typedef struct kl_paged_attention_args {
+  const void* q;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  long long q_row_stride, q_head_stride, table_stride;
+  kl_kv_cache cache;
+  int dtype, batch, heads, columns;
+  float scale;
+} kl_paged_attention_args;
+int kl_paged_attention(const kl_paged_attention_args* args, void* stream);
 
 /*
  * Host-only description of the launch plan kl_linear would use on a device

@@ -530,11 +530,13 @@ def test_c_abi_rejects_bad_arguments_without_a_gpu():
         return N.KV_CACHE.pack(k, v, ks, vs, *strides, 32, 16, 1, fmt, pages, page, heads, dim)
 
     def attend(c=None, q=fake, dtype=N.KL_DT_BF16, batch=1, heads=4, columns=2, lengths=fake, scale=1.0, out=fake, table=fake):
-        return lib.kl_paged_attention(q, 512, 128, dtype, batch, heads, c or cache(), table, 2, columns, lengths, scale, out, None,
-                                      None, 0, None)
+        args = N.PAGED_ATTENTION_ARGS.pack(q or 0, table or 0, lengths or 0, out or 0, 0, 0, 0, 512, 128, 2, c or cache(), dtype, batch,
+                                           heads, columns, scale)
+        return lib.kl_paged_attention(args, None)
 
     bad = N.KL_ERR_INVALID
     assert lib.kl_read_kv(None, N.KL_DT_BF16, fake, 1, fake, fake, None) == bad
+    assert lib.kl_paged_attention(None, None) == bad and lib.kl_qk_norm_rope_write(None, None) == bad
     for c in (cache(k=0), cache(k=8), cache(strides=(4096, 2048, 132)), cache(fmt=2), cache(fmt=N.KL_KV_INT8), cache(pages=0),
               cache(page=0), cache(heads=0), cache(dim=96)):
         assert attend(c) == bad and lib.kl_read_kv(c, N.KL_DT_BF16, fake, 1, fake, fake, None) == bad
@@ -546,8 +548,9 @@ def test_c_abi_rejects_bad_arguments_without_a_gpu():
     assert attend(batch=0) == N.KL_OK
 
     def write(c=None, tokens=1, heads=4, qw=fake, kw=fake, rows=8, eps=1e-6, q=fake, slots=fake, dtype=N.KL_DT_BF16):
-        return lib.kl_qk_norm_rope_write(q, 512, 128, fake, 256, 128, fake, 256, 128, dtype, tokens, heads, qw, kw, fake, fake, rows,
-                                         fake, slots, eps, c or cache(), fake, None)
+        args = N.KV_WRITE_ARGS.pack(q or 0, fake, fake, qw or 0, kw or 0, fake, fake, fake, slots or 0, fake, 512, 128, 256, 128, 256, 128,
+                                    c or cache(), dtype, tokens, heads, rows, eps)
+        return lib.kl_qk_norm_rope_write(args, None)
 
     assert write(tokens=-1) == bad and write(heads=0) == bad and write(kw=None) == bad and write(rows=0) == bad
     assert write(eps=0.0) == bad and write(eps=float("nan")) == bad and write(q=None) == bad and write(slots=None) == bad
