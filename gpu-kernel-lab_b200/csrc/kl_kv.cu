@@ -128,10 +128,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvWriteArgs 
 struct Slot {
   int64_t page, off;
 };
-KL_DEVICE Slot split_slot(int64_t slot, int page_size) {
-  if (static_cast<uint64_t>(slot) >> 32) return {slot / page_size, slot % page_size};
-  const uint32_t s = static_cast<uint32_t>(slot), p = s / static_cast<uint32_t>(page_size);
-  return {p, s - p * page_size};
+KL_DEVICE Slot split_slot(int64_t slot, const KvView& kv) {
+  if (static_cast<uint64_t>(slot) >> 31) return {slot / kv.page_size, slot % kv.page_size};
+  const uint32_t s = static_cast<uint32_t>(slot), p = page_of(kv, s);
+  return {p, s - p * kv.page_size};
 }
 
 // 32 bytes of one lane at a 32-byte boundary: one instruction, so that every sector is written whole
@@ -269,7 +269,10 @@ __global__ void __launch_bounds__(kKvThreads, kWriteBlocks) kv_write_vec_kernel(
     fetch(stage == 0 ? kWriteStages - 1 : stage - 1);
     stage = stage == kWriteStages - 1 ? 0 : stage + 1;
   };
+  // u' = inv (u uc + v vs),  v' = inv (v vc + u us)
+  f32x2 uc[4], us[4], vc[4], vs[4];
   for (; todo > 0; ++token, p = 0) {
+    bool turned = false;                                    // the rotation is the token's; without norms keys take the queries'
     int64_t pos = next_pos;
     if (pos < 0 || pos >= a.max_positions) {
       record_error(a.status, KL_ERR_INVALID);
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(kKvThreads, kWriteBlocks) kv_write_vec_kernel(
     }
     const bool cached = next_slot >= 0 && next_slot < room;
     if (next_slot >= room) record_error(a.status, KL_ERR_INVALID);
-    const Slot at = split_slot(cached ? next_slot : 0, a.kv.page_size);
+    const Slot at = split_slot(cached ? next_slot : 0, a.kv);
     if (token + 1 < a.tokens) {
       next_pos = a.positions[token + 1];
       next_slot = a.slots[token + 1];
@@ -299,9 +302,8 @@ __global__ void __launch_bounds__(kKvThreads, kWriteBlocks) kv_write_vec_kernel(
         out = (kind == 1 ? a.kv.k : a.kv.v) + (to + head * a.kv.head_stride) * (INT8 ? 1 : 2);
         inc = R * a.kv.head_stride * (INT8 ? 1 : 2);
       }
-      // u' = inv (u uc + v vs),  v' = inv (v vc + u us)
-      f32x2 uc[4], us[4], vc[4], vs[4];
-      if constexpr (kind < 2) {
+      if (kind < 2 && !(turned && !a.weight[0])) {
+        turned = true;
         const float4* c = reinterpret_cast<const float4*>(a.cos + pos * (D / 2) + 8 * j);
         const float4* s = reinterpret_cast<const float4*>(a.sin + pos * (D / 2) + 8 * j);
 #pragma unroll
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(kKvThreads, kWriteBlocks) kv_write_vec_kernel(
           vs[2 * i + 1] = pair(-y.z, -y.w);
         }
         if (a.weight[0]) {
-          const T* wt = static_cast<const T*>(a.weight[kind]) + 8 * j;
+          const T* wt = static_cast<const T*>(a.weight[kind == 1 ? 1 : 0]) + 8 * j;
           f32x2 wu[4], wv[4];
           unpack8<T>(wu, __ldg(reinterpret_cast<const uint4*>(wt)));
           unpack8<T>(wv, __ldg(reinterpret_cast<const uint4*>(wt + D / 2)));
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_vec_kernel(const KvView kv
   uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
   float scale[2] = {0.0f, 0.0f};
   if (there) {
-    const Slot at = split_slot(slot, kv.page_size);
+    const Slot at = split_slot(slot, kv);
     const int64_t from = (at.page * kv.page_stride + head * kv.head_stride + at.off * kv.token_stride) * static_cast<int>(sizeof(C)) + 16 * j;
     raw[0] = __ldcs(reinterpret_cast<const uint4*>(kv.k + from));
     raw[1] = __ldcs(reinterpret_cast<const uint4*>(kv.v + from));
@@ -515,6 +517,12 @@ KvView kv_view(const kl_kv_cache& c) {
   v.pages = c.pages;
   v.page_size = c.page_size;
   v.kv_heads = c.kv_heads;
+  // with 2^log >= page_size, page_mul * page_size = 2^(31 + log) + e, e < 2^log: for x < 2^31 the
+  // product exceeds x / page_size by less than 1 / page_size
+  int log = 0;
+  while ((1ll << log) < c.page_size) ++log;
+  v.page_mul = static_cast<uint32_t>(((1ull << (31 + log)) + c.page_size - 1) / c.page_size);
+  v.page_shift = 31 + log;
   v.page_stride = c.page_stride;
   v.head_stride = c.head_stride;
   v.token_stride = c.token_stride;

@@ -16,9 +16,15 @@ struct KvView {
   float* ks;                       // int8 only: one scale per (page, head, token)
   float* vs;
   int pages, page_size, kv_heads;
+  uint32_t page_mul;               // x / page_size = x * page_mul >> page_shift for x < 2^31
+  int page_shift;
   long long page_stride, head_stride, token_stride;          // elements
   long long s_page_stride, s_head_stride, s_token_stride;
 };
+
+KL_DEVICE uint32_t page_of(const KvView& kv, uint32_t x) {
+  return static_cast<uint32_t>(static_cast<uint64_t>(x) * kv.page_mul >> kv.page_shift);
+}
 
 template <typename T> KL_DEVICE float kv_to_f(T v);
 template <> KL_DEVICE float kv_to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -72,8 +72,6 @@ struct AttnArgs {
   int blocks;                          // blocks of HB query heads per KV head
   int q_vec;                           // q rows allow 4-byte loads
   int box;                             // rows of one TMA box (divides the page), 0: copies by the lanes
-  uint32_t page_mul;                   // position / page_size = position * page_mul >> page_shift
-  int page_shift;
   float scale;
   void* out;
   float* lse;
@@ -371,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
 #pragma unroll
     for (int w = 0; w < kWords; ++w) {
       const int row = w * 32 + lane, pos = pos0 + row;
-      const unsigned column = static_cast<unsigned>(static_cast<uint64_t>(static_cast<unsigned>(pos)) * a.page_mul >> a.page_shift);
+      const unsigned column = page_of(a.kv, pos);
       rest[w] = pos - column * a.kv.page_size;
       page[w] = row < G::kKeys && pos < in.len ? __ldg(table + column) : 0;
     }
@@ -978,10 +976,6 @@ cudaError_t launch_paged_attention(const kl_paged_attention_args& p, int sm_coun
   const int hb = heads_per_cta(a.group, dim);
   a.blocks = (a.group + hb - 1) / hb;
   a.q_vec = (reinterpret_cast<uintptr_t>(p.q) % 4 == 0) && p.q_row_stride % 2 == 0 && p.q_head_stride % 2 == 0;
-  int log = 0;
-  while ((1ll << log) < p.cache.page_size) ++log;
-  a.page_mul = static_cast<uint32_t>(((1ull << (31 + log)) + p.cache.page_size - 1) / p.cache.page_size);
-  a.page_shift = 31 + log;
   a.scale = p.scale;
   a.out = p.out;
   a.lse = p.lse;
