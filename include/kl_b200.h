@@ -23,6 +23,9 @@
  *                            and its asymmetric bf16 scale/zero sibling (KL_W4_ASYM)
  *   kl_dequantize         <- learning/10_cuda_decode/activation_int8.py:63-64 dequantize_int8,
  *                            learning/09_int4/quantization.py:65-71 dequantize_int4
+ *   kl_qk_norm_rope_write <- learning/08_decode/fused_qkv_cache.py:7-54 (on a paged cache)
+ *   kl_paged_attention    <- serving/paged_attention.py:11-101
+ *   kl_read_kv            <- serving/paged_gather.py:8-28
  */
 #ifndef KL_B200_H
 #define KL_B200_H
