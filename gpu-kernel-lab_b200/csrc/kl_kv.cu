@@ -212,6 +212,8 @@ __global__ void __launch_bounds__(kKvThreads, kWriteBlocks) kv_write_vec_kernel(
   const int lane = threadIdx.x & 31, j = lane % LANES, sub = lane / LANES;
   const int q_passes = (a.heads + R - 1) / R, kv_passes = (a.kv.kv_heads + R - 1) / R, passes = q_passes + 2 * kv_passes;
   // this warp's steps [lo, hi) of tokens * passes
+  pdl_wait();
+  pdl_launch_dependents();
   const uint32_t warps = gridDim.x * (kKvThreads / 32), w = (threadIdx.x >> 5) * gridDim.x + blockIdx.x;
   const uint64_t steps = static_cast<uint64_t>(a.tokens) * passes;
   const uint32_t lo = static_cast<uint32_t>(steps * w / warps), hi = static_cast<uint32_t>(steps * (w + 1) / warps);
@@ -427,6 +429,8 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_vec_kernel(const KvView kv
                                                                  T* __restrict__ k, T* __restrict__ v, int* status) {
   using C = typename std::conditional<INT8, int8_t, T>::type;
   constexpr int E = 16 / sizeof(C), LANES = D / E;
+  pdl_wait();
+  pdl_launch_dependents();
   const uint32_t j = threadIdx.x % LANES, item = blockIdx.x * (kKvThreads / LANES) + threadIdx.x / LANES;
   if (item >= pairs) return;
   const uint32_t token = item / kv.kv_heads, head = item - token * kv.kv_heads;
@@ -477,10 +481,9 @@ cudaError_t write_t(const KvWriteArgs& a, int sm_count, cudaStream_t s) {
     constexpr int R = 32 / (D / 16);
     const long long steps = a.tokens * ((a.heads + R - 1) / R + 2ll * ((a.kv.kv_heads + R - 1) / R));
     const unsigned grid = static_cast<unsigned>(std::min((steps + 7) / 8, static_cast<long long>(kWriteBlocks) * sm_count));
-    kv_write_vec_kernel<T, INT8, D / 16><<<grid, kKvThreads, 0, s>>>(a);
-  } else {
-    kv_write_kernel<T, INT8, D / 32><<<static_cast<unsigned>((a.tokens * rows + 7) / 8), kKvThreads, 0, s>>>(a);
+    return launch_dependent(kv_write_vec_kernel<T, INT8, D / 16>, dim3(grid), kKvThreads, 0, s, a);
   }
+  kv_write_kernel<T, INT8, D / 32><<<static_cast<unsigned>((a.tokens * rows + 7) / 8), kKvThreads, 0, s>>>(a);
   return cudaGetLastError();
 }
 template <typename T, bool INT8>
@@ -495,8 +498,8 @@ cudaError_t read_t(const KvView& kv, const int64_t* slots, int tokens, void* k, 
   constexpr int kPairs = kKvThreads / (D * (INT8 ? 1 : 2) / 16);       // pairs of one block
   const uint32_t pairs = static_cast<uint32_t>(tokens) * kv.kv_heads;
   const uint32_t grid = (pairs + kPairs - 1) / kPairs;
-  kv_read_vec_kernel<T, INT8, D><<<grid, kKvThreads, 0, s>>>(kv, slots, pairs, static_cast<T*>(k), static_cast<T*>(v), status);
-  return cudaGetLastError();
+  return launch_dependent(kv_read_vec_kernel<T, INT8, D>, dim3(grid), kKvThreads, 0, s, kv, slots, pairs, static_cast<T*>(k),
+                          static_cast<T*>(v), status);
 }
 template <typename T, bool INT8>
 cudaError_t read_d(const KvView& kv, int head_dim, const int64_t* slots, int tokens, void* k, void* v, int* status, int sm_count,

@@ -83,4 +83,21 @@ KL_DEVICE float kv_warp_max(float v) {
   return v;
 }
 
+// Launch as a programmatic dependent of the kernel before: the launch is under way when that ends. The
+// kernel waits for that kernel's end (pdl_wait) before it touches what other kernels write.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A&&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 }  // namespace kl

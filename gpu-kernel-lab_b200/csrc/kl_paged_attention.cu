@@ -245,8 +245,10 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   const int t4 = lane & 3, l4 = lane >> 2;
   const int rows = a.kv.kv_heads * a.blocks;        // rows per sequence
 
-  // what the first units will wait for is brought into L2
+  if (tid < kWarps * kStages) mbar_init(smem_u32(bars + tid), a.box ? 1 : 33);
   if (tid == 0) {
+    fence_mbar_init();
+    s_piece->ways = 0;
     prefetch_tmap(&maps.k);
     prefetch_tmap(&maps.v);
     if constexpr (INT8) {
@@ -254,6 +256,9 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
       prefetch_tmap(&maps.vs);
     }
   }
+  pdl_wait();                                       // up to here nothing was read that another kernel writes
+  pdl_launch_dependents();
+  // what the first units will wait for is brought into L2
   if (blockIdx.x < a.batch && tid * 32 < a.columns) prefetch_l2(a.table + blockIdx.x * a.table_stride + tid * 32);
   if (blockIdx.x < a.batch && tid < a.heads * (D / 64))
     prefetch_l2(static_cast<const char*>(a.q) + (blockIdx.x * a.q_row_stride + tid / (D / 64) * a.q_head_stride) * 2 + tid % (D / 64) * 128);
@@ -282,9 +287,6 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   }
   int* s_tot = s_misc;
   if (lane == 31) s_tot[warp] = incl;
-  if (tid < kWarps * kStages) mbar_init(smem_u32(bars + tid), a.box ? 1 : 33);
-  if (tid == 0) fence_mbar_init();
-  if (tid == 0) s_piece->ways = 0;
   __syncthreads();
   int total = 0;
 #pragma unroll
@@ -816,6 +818,7 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinBlocks) join_kernel(const P
   __shared__ float4 s_v[kSides][kVecs];
   __shared__ float s_m[kSides][kVecs], s_l[kSides][kVecs];
   pdl_wait();
+  pdl_launch_dependents();
   const int side = threadIdx.x / kVecs, vec = threadIdx.x % kVecs;
   const int col = blockIdx.y * kHeads + vec / (D / 4), d = vec % (D / 4) * 4;
   for (int c = blockIdx.x; c < count; c += gridDim.x) {
@@ -933,19 +936,11 @@ cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   char* const space = static_cast<char*>(a.workspace) + kCounterBytes;
   a.records = room > kWholeUnits * G::kUnit ? reinterpret_cast<Piece*>(space) : nullptr;
   a.partials = reinterpret_cast<float*>(space + kRecordBytes);
-  attn_kernel<T, INT8, D, HB><<<grid, kThreads, G::kSmem, s>>>(a, maps);
-  if ((e = cudaGetLastError()) != cudaSuccess || !a.records) return e;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(std::min<unsigned>(grid, kJoinBlocks * sm_count), (std::min(a.group, HB) + join_heads(HB) - 1) / join_heads(HB));
-  config.blockDim = dim3(kJoinThreads);
-  config.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, join_kernel<T, D, HB>, static_cast<const Piece*>(a.records), static_cast<int>(grid), static_cast<const float*>(a.partials),
-                            static_cast<T*>(a.out), a.lse);
+  e = launch_dependent(attn_kernel<T, INT8, D, HB>, dim3(grid), kThreads, G::kSmem, s, a, maps);
+  if (e != cudaSuccess || !a.records) return e;
+  const unsigned parts = (std::min(a.group, HB) + join_heads(HB) - 1) / join_heads(HB);
+  return launch_dependent(join_kernel<T, D, HB>, dim3(std::min<unsigned>(grid, kJoinBlocks * sm_count), parts), kJoinThreads, 0, s,
+                          a.records, static_cast<int>(grid), a.partials, static_cast<T*>(a.out), a.lse);
 }
 
 // Query heads of one CTA: all of a KV head's where they fit, so that its keys are read and converted once. 16 instead of
