@@ -123,7 +123,7 @@ LENGTHS = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 129, 200, 511, 1000, 40
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("quantized", [False, True])
-@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 8, 128), (8, 8, 64), (6, 2, 128), (4, 1, 256), (32, 2, 128), (17, 1, 64), (40, 1, 128)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 8, 128), (8, 8, 64), (6, 2, 128), (4, 1, 256), (32, 2, 128), (17, 1, 64), (40, 1, 128), (12, 1, 256)])
 def test_attention_over_ragged_lengths(dtype, quantized, heads, kv_heads, dim):
     check_attention(*batch(generator(heads + dim), TYPES[dtype], quantized, heads, kv_heads, dim, 16, LENGTHS))
 
@@ -137,7 +137,7 @@ def test_attention_over_page_sizes(quantized, page):
 
 @gpu
 @pytest.mark.parametrize("quantized", [False, True])
-@pytest.mark.parametrize("lengths", [[1], [37], [64], [65], [20000], [0], [0, 0, 0], [3000] * 3, [1] * 700, [0, 16000] + [5] * 300])
+@pytest.mark.parametrize("lengths", [[1], [37], [64], [65], [20000], [0], [0, 0, 0], [3000] * 3, [1] * 700, [0, 16000] + [5] * 300, [5, 300] * 300 + [3000]])
 def test_attention_of_few_and_many_sequences(quantized, lengths):
     check_attention(*batch(generator(len(lengths)), torch.bfloat16, quantized, 6, 2, 128, 16, lengths))
 
