@@ -43,6 +43,8 @@ HEAD_DIMS = (64, 128, 256)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _empty_here = getattr(torch._C._dynamo.guards, "_empty_strided_cuda", None)
+_is_compiling = torch.compiler.is_compiling
+_I8, _I32, _I64, _F32 = torch.int8, torch.int32, torch.int64, torch.float32
 _CODES = {torch.bfloat16: N.KL_DT_BF16, torch.float16: N.KL_DT_F16}
 
 
@@ -87,29 +89,29 @@ def _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index):
     pages, kv_heads, page_size, head_dim = shape
     if head_dim not in HEAD_DIMS:
         raise ValueError('head_dim must be 64, 128 or 256')
-    if v_cache.dtype != held:
+    if v_cache.dtype is not held:
         raise ValueError('k_cache and v_cache must have one dtype')
-    if held == torch.int8:
+    if held is _I8:
         if k_scales is None or v_scales is None:
             raise ValueError('an int8 cache needs k_scales and v_scales')
         scale_strides = k_scales.stride()
         if k_scales.shape != shape[:3] or v_scales.shape != shape[:3] or v_scales.stride() != scale_strides:
             raise ValueError('scales must be [pages, kv_heads, page_size] with equal strides')
-        if (k_scales.dtype != torch.float32 or v_scales.dtype != torch.float32 or k_scales.get_device() != index
+        if (k_scales.dtype is not _F32 or v_scales.dtype is not _F32 or k_scales.get_device() != index
                 or v_scales.get_device() != index):
             raise ValueError('scales must be FP32 on the cache\'s device')
         return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), strides[0],
                                strides[1], strides[2], *scale_strides, N.KL_KV_INT8, pages, page_size, kv_heads, head_dim)
     if k_scales is not None or v_scales is not None:
         raise ValueError('only an int8 cache has scales')
-    if held != dtype:
+    if held is not dtype:
         raise ValueError('the cache must be int8 or of the activations\' dtype')
     return N.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, strides[0], strides[1], strides[2], 0, 0, 0, N.KL_KV_SAME,
                            pages, page_size, kv_heads, head_dim)
 
 
 def _check_vector(t, name, dtype, count, index):
-    if t.dtype != dtype or t.shape != (count,) or t.get_device() != index or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (count,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f'{name} must be a contiguous {dtype} vector of {count} on the cache\'s device')
 
 
@@ -149,7 +151,7 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
 
     The arithmetic is f32 up to one rounding at the store (an int8 cache quantises the f32 value).
     """
-    if torch.compiler.is_compiling():
+    if _is_compiling():
         return torch.ops.kl_b200.qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache,
                                                     k_scales, v_scales, epsilon)
     shape, kv_shape = q.shape, k.shape
@@ -157,7 +159,7 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
         raise ValueError('q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]')
     tokens, heads, dim = shape
     dtype, index = q.dtype, q.get_device()
-    if dtype not in _CODES or k.dtype != dtype or v.dtype != dtype:
+    if dtype not in _CODES or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError('q, k and v must have matching FP16/BF16 dtype')
     if index < 0 or k.get_device() != index or v.get_device() != index:
         raise ValueError('q, k, v and the cache must be on the same CUDA device')
@@ -179,11 +181,11 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
     table = cos.shape
     if len(table) != 2 or table[0] == 0 or 2 * table[1] != dim or sin.shape != table:
         raise ValueError('cos and sin must be [max_positions, head_dim / 2]')
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.get_device() != index or sin.get_device() != index
+    if (cos.dtype is not _F32 or sin.dtype is not _F32 or cos.get_device() != index or sin.get_device() != index
             or not cos.is_contiguous() or not sin.is_contiguous()):
         raise ValueError('cos and sin must be contiguous FP32 on the cache\'s device')
-    _check_vector(positions, 'positions', torch.int64, tokens, index)
-    _check_vector(slots, 'slots', torch.int64, tokens, index)
+    _check_vector(positions, 'positions', _I64, tokens, index)
+    _check_vector(slots, 'slots', _I64, tokens, index)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError('inference only; use torch.inference_mode()')
     out = _empty(q, (tokens, heads, dim), dtype, index)
@@ -200,16 +202,16 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
 
     ``dtype`` (bf16 or f16) is that of the result of an int8 cache, bf16 if not given; a 16-bit cache returns its own.
     """
-    if torch.compiler.is_compiling():
+    if _is_compiling():
         return torch.ops.kl_b200.read_kv(k_cache, v_cache, slots, k_scales, v_scales, dtype)
     if dtype is None:
-        dtype = torch.bfloat16 if k_cache.dtype == torch.int8 else k_cache.dtype
+        dtype = torch.bfloat16 if k_cache.dtype is _I8 else k_cache.dtype
     if dtype not in _CODES:
         raise ValueError('keys and values are read as FP16/BF16')
     index = slots.get_device()
     cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index)
     tokens = slots.numel()
-    _check_vector(slots, 'slots', torch.int64, tokens, index)
+    _check_vector(slots, 'slots', _I64, tokens, index)
     shape = (tokens, k_cache.shape[1], k_cache.shape[3])
     k, v = _empty(k_cache, shape, dtype, index), _empty(k_cache, shape, dtype, index)
     if tokens:
@@ -231,7 +233,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     exponentials (``-inf`` for a length of 0), by which parts of a sequence can be joined.  ``workspace`` (uint8, zeroed
     once, of ``paged_attention_workspace_bytes``) takes the place of the scratch kept per device and stream.
     """
-    if torch.compiler.is_compiling():
+    if _is_compiling():
         both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale)
         return both if return_lse else both[0]
     shape = q.shape
@@ -251,12 +253,12 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     if dim != k_cache.shape[3] or heads == 0 or heads % kv_heads:
         raise ValueError('q must match the cache\'s head_dim and have a multiple of its heads')
     table = page_table.shape
-    if len(table) != 2 or table[0] != batch or page_table.dtype != torch.int32 or page_table.get_device() != index:
+    if len(table) != 2 or table[0] != batch or page_table.dtype is not _I32 or page_table.get_device() != index:
         raise ValueError('page_table must be int32 [batch, columns] on the cache\'s device')
     table_stride, step = page_table.stride()
     if step != 1 and table[1] > 1:
         raise ValueError('page_table must have contiguous rows')
-    _check_vector(lengths, 'lengths', torch.int32, batch, index)
+    _check_vector(lengths, 'lengths', _I32, batch, index)
     if scale is None:
         scale = dim ** -0.5
     elif not math.isfinite(scale):
