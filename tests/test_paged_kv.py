@@ -247,6 +247,38 @@ def test_attention_on_another_stream_and_in_a_graph():
 
 
 @gpu
+def test_captured_behind_copies_and_memsets():
+    """In a graph every launch waits for what comes before it, copies and memsets too, and for the operators among each other."""
+    q, cache, table, lengths = batch(generator(18), torch.bfloat16, False, 4, 2, 128, 16, [2000, 33], poison=False)
+    k, v = (torch.randn(2, 2, 128, generator=generator(19), device="cuda").bfloat16() for _ in range(2))
+    cos, sin = rope_tables(None, 128, cache.k_cache.shape[0] * 16)
+    lens, slots, new = torch.zeros_like(lengths), torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros_like(v)
+    space = torch.zeros(kl.paged_attention_workspace_bytes(2, 4, 2, 128), dtype=torch.uint8, device="cuda")
+    wanted = kl.kv_slots(table, torch.arange(2, device="cuda"), lengths.long() - 1, 16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        slots.copy_(wanted)
+        new.zero_()
+        lens.copy_(lengths)
+        turned = kl.qk_norm_rope_write(q, k, new, None, None, cos, sin, slots, slots, *cache)
+        first = kl.paged_attention(turned, cache.k_cache, cache.v_cache, table, lens, workspace=space)
+        new.copy_(v)
+        turned = kl.qk_norm_rope_write(q, k, new, None, None, cos, sin, slots, slots, *cache)
+        second = kl.paged_attention(turned, cache.k_cache, cache.v_cache, table, lens, workspace=space)
+        got = kl.read_kv(cache.k_cache, cache.v_cache, slots)[1]
+    for _ in range(20):
+        lens.zero_()
+        slots.fill_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, v)
+        ref = kl.qk_norm_rope_write(q, k, torch.zeros_like(v), None, None, cos, sin, slots, slots, *cache)
+        assert torch.equal(first, kl.paged_attention(ref, cache.k_cache, cache.v_cache, table, lengths))
+        kl.qk_norm_rope_write(q, k, v, None, None, cos, sin, slots, slots, *cache)
+        assert torch.equal(second, kl.paged_attention(ref, cache.k_cache, cache.v_cache, table, lengths))
+
+
+@gpu
 def test_attention_out_of_range_table_is_recorded_not_read():
     q, cache, table, lengths = batch(generator(5), torch.bfloat16, False, 4, 2, 128, 16, [40, 40, 40], poison=False)
     ref = kl.paged_attention(q, cache.k_cache, cache.v_cache, table, lengths)
