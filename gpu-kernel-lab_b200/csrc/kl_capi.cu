@@ -971,9 +971,9 @@ int kl_paged_attention(const kl_paged_attention_args* args, void* stream) {
   const long long room = static_cast<long long>(a.columns) * c.page_size;
   if (room > 0x7FFF0000ll || static_cast<long long>(a.batch) * a.heads > 0x7FFFFFFFll)
     return fail(KL_ERR_INVALID, "columns * page_size and batch * heads must stay below 2^31");
-  // units of at least 64 keys; the kernel counts them in 32 bits
-  if (static_cast<long long>(a.batch) * a.heads * ((room + 63) / 64) > 0x7FFFFFFFll)
-    return fail(KL_ERR_INVALID, "batch * heads * columns * page_size / 64 must stay below 2^31");
+  // units of at least 64 keys, and one more for a row; the kernel counts them in 32 bits
+  if (static_cast<long long>(a.batch) * a.heads * ((room + 63) / 64 + 1) > 0x7FFFFFFFll)
+    return fail(KL_ERR_INVALID, "batch * heads * (columns * page_size / 64 + 1) must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
   const size_t need = paged_attention_workspace_bytes(a.heads, c.kv_heads, c.head_dim, di.sm_count);

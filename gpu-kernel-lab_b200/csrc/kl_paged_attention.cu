@@ -270,6 +270,9 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     return n < 0 ? 0 : static_cast<int>(n < room ? n : room);
   };
   auto units_of = [&](int n) { return (n + G::kUnit - 1) / G::kUnit; };
+  // what a row counts for in the partition: its units, and one more for its begin and end where rows stay whole (256
+  // requests of 1 to 250 tokens: 32.4 us against 39.8 by units alone)
+  auto weight_of = [&](int n) { return n > 0 ? units_of(n) + (a.records ? 0 : 1) : 0; };
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
   int mine = 0;
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     const int n = length_of(b);
     if (a.lengths[b] > room) record_error(a.status, KL_ERR_INVALID);
     if (b < kMaxLens) s_len[b] = n;
-    mine += units_of(n);
+    mine += weight_of(n);
   }
   int incl = mine;
 #pragma unroll
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     if ((end == 0 || !a.records) && (incl - mine) * rows <= u && u < incl * rows) {
       int before = (incl - mine) * rows, b = b0;
       for (;; ++b) {
-        const int n = units_of(length_of(b)) * rows;
+        const int n = weight_of(length_of(b)) * rows;
         if (u < before + n) break;
         before += n;
       }
@@ -348,8 +351,9 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   Cursor in;                                        // next unit to fetch
   in.b = s_misc[8];
   load_len(in);
-  in.head = s_misc[9] / in.units;
-  in.i = s_misc[9] - in.head * in.units;
+  const int weight = weight_of(in.len);
+  in.head = s_misc[9] / weight;
+  in.i = s_misc[9] - in.head * weight;
   in.block = 0;
   if (a.blocks > 1) {
     in.block = in.head % a.blocks;
@@ -357,15 +361,22 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   }
   if (!a.records) {                                 // whole rows: those that begin in [lo, hi)
     if (hi < total) {
-      const int units = units_of(s_misc[10] < kMaxLens ? s_len[s_misc[10]] : length_of(s_misc[10])), over = s_misc[11] % units;
-      if (over) count += units - over;
+      const int last = weight_of(s_misc[10] < kMaxLens ? s_len[s_misc[10]] : length_of(s_misc[10])), over = s_misc[11] % last;
+      if (over) count += last - over;
     }
     if (in.i > 0) {
-      count -= in.units - in.i;
+      count -= weight - in.i;
       in.i = in.units - 1;
       if (count > 0) advance(in);
     }
     if (count <= 0) return;
+    Cursor row = in;                                // from weights to units
+    for (int left = count; left > 0;) {
+      left -= row.units + 1;
+      --count;
+      row.i = row.units - 1;
+      if (left > 0) advance(row);
+    }
   }
   Cursor at = in;                                   // unit being computed
 
