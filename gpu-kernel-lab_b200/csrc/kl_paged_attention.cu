@@ -14,7 +14,8 @@
 // are only read on the device, so a captured launch serves any lengths. A row
 // that crosses CTAs leaves partial (maximum, sum, output) triples in the
 // workspace, and a dependent launch joins them in CTA order: results do not
-// depend on timing.
+// depend on timing. Rows that are short, or many, are not split at all (the rule is
+// at kWholeUnits).
 //
 // CTA. Four warps, each with its own keys of a unit and its own ring of kStages
 // shared-memory slots of 8 KB, filled by TMA: one box per page (or per
@@ -64,6 +65,11 @@ constexpr int join_heads(int hb) { return hb == 16 ? 4 : 2; }   // heads of one 
 // it is shorter there too (192 f16 requests of up to 301 tokens: 19.5 against 22.3). 8 units: 14.0 us against 9.0
 // (8 requests of 500 tokens).
 constexpr int kWholeUnits = 4;
+// Nor are rows of up to so many units where there are two waves of rows and more: 128 requests of 1 to 500 tokens on 8
+// heads took 31.9 us against 40.5 split, of 1 to 1000 tokens 53.1 against 64.4, 256 of 1 to 2000 (32 units) 178.9 against
+// 180.2; with 1.2 waves (64 requests of 100 to 500 tokens) 23.2 against 21.4. The bound limits what one long row
+// among short ones can cost.
+constexpr int kWholeUnitsOfMany = 16;
 constexpr int kMaxLens = 512;          // lengths kept in shared memory
 constexpr float kSlack = 8.0f;           // log2 of how far weights may exceed 1
 constexpr float kLog2e = 1.4426950408889634f;
@@ -941,11 +947,12 @@ cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
     allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
   const long long room = static_cast<long long>(a.columns) * a.kv.page_size;
-  const long long most = static_cast<long long>(a.batch) * a.kv.kv_heads * a.blocks * ((room + G::kUnit - 1) / G::kUnit);
+  const long long rows = static_cast<long long>(a.batch) * a.kv.kv_heads * a.blocks, most = rows * ((room + G::kUnit - 1) / G::kUnit);
   const long long wave = static_cast<long long>(sm_count) * G::kResident;
+  const bool whole = room <= (rows >= 2 * wave ? kWholeUnitsOfMany : kWholeUnits) * G::kUnit;
   const unsigned grid = static_cast<unsigned>(std::max(1ll, std::min({most, wave, static_cast<long long>(kMaxCtas)})));
   char* const space = static_cast<char*>(a.workspace) + kCounterBytes;
-  a.records = room > kWholeUnits * G::kUnit ? reinterpret_cast<Piece*>(space) : nullptr;
+  a.records = whole ? nullptr : reinterpret_cast<Piece*>(space);
   a.partials = reinterpret_cast<float*>(space + kRecordBytes);
   e = launch_dependent(attn_kernel<T, INT8, D, HB>, dim3(grid), kThreads, G::kSmem, s, a, maps);
   if (e != cudaSuccess || !a.records) return e;

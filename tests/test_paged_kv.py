@@ -144,6 +144,15 @@ def test_attention_of_few_and_many_sequences(quantized, lengths):
 
 @gpu
 @pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("longest", [250, 990])
+def test_attention_of_many_rows(quantized, longest):
+    """More rows than two waves of CTAs, of very different lengths, some empty."""
+    lengths = [(i * i * 37) % (longest + 1) if i % 9 else 0 for i in range(130)] + [longest]
+    check_attention(*batch(generator(longest), torch.bfloat16, quantized, 16, 8, 64, 16, lengths))
+
+
+@gpu
+@pytest.mark.parametrize("quantized", [False, True])
 def test_attention_strides(quantized):
     """A cache laid out by token, queries inside a fused row, a table inside a wider one."""
     g = generator(3)
