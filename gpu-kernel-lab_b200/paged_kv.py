@@ -115,10 +115,10 @@ def _check_vector(t, name, dtype, count, index):
         raise ValueError(f'{name} must be a contiguous {dtype} vector of {count} on the cache\'s device')
 
 
-def _empty(like, shape, dtype, index):
-    """An uninitialised contiguous tensor of three dimensions on CUDA device ``index``, that of ``like``."""
+def _empty(like, shape, strides, dtype, index):
+    """An uninitialised tensor on CUDA device ``index``, that of ``like``; ``strides`` are a contiguous tensor's."""
     if _empty_here is not None and index == _current_device():
-        return _empty_here(shape, (shape[1] * shape[2], shape[2], 1), dtype)
+        return _empty_here(shape, strides, dtype)
     return like.new_empty(shape, dtype=dtype)
 
 
@@ -188,7 +188,7 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
     _check_vector(slots, 'slots', _I64, tokens, index)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise ValueError('inference only; use torch.inference_mode()')
-    out = _empty(q, (tokens, heads, dim), dtype, index)
+    out = _empty(q, (tokens, heads, dim), (heads * dim, dim, 1), dtype, index)
     if tokens:
         args = N.KV_WRITE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_weight_at, k_weight_at, cos.data_ptr(),
                                     sin.data_ptr(), positions.data_ptr(), slots.data_ptr(), out.data_ptr(), sq[0], sq[1], sk[0],
@@ -212,8 +212,9 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
     cache = _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index)
     tokens = slots.numel()
     _check_vector(slots, 'slots', _I64, tokens, index)
-    shape = (tokens, k_cache.shape[1], k_cache.shape[3])
-    k, v = _empty(k_cache, shape, dtype, index), _empty(k_cache, shape, dtype, index)
+    _, kv_heads, _, dim = k_cache.shape
+    shape, strides = (tokens, kv_heads, dim), (kv_heads * dim, dim, 1)
+    k, v = _empty(k_cache, shape, strides, dtype, index), _empty(k_cache, shape, strides, dtype, index)
     if tokens:
         _call(index, N.lib().kl_read_kv, cache, _CODES[dtype], slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr())
     return k, v
@@ -265,8 +266,8 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
         raise ValueError('scale must be finite')
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError('inference only; use torch.inference_mode()')
-    out = _empty(q, (batch, heads, dim), dtype, index)
-    lse = q.new_empty((batch, heads), dtype=torch.float32) if return_lse else None
+    out = _empty(q, (batch, heads, dim), (heads * dim, dim, 1), dtype, index)
+    lse = _empty(q, (batch, heads), (heads, 1), _F32, index) if return_lse else None
     if batch:
         if workspace is None:
             workspace = N.workspace(q.device, paged_attention_workspace_bytes(1, heads, kv_heads, dim), _raw_stream(index))
