@@ -40,9 +40,9 @@ HEAD_DIMS = (64, 128, 256)
 # A call of one token is as long as its host side, so three calls take torch's shorter ways: the current stream
 # as an integer (torch.cuda.current_stream() takes 2 us), the current device, and an allocation on it (0.9 us, 1.5 to 2.5 by
 # empty_like, new_empty or torch.empty).
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
-_empty_here = getattr(torch._C._dynamo.guards, "_empty_strided_cuda", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 _is_compiling = torch.compiler.is_compiling
 _I8, _I32, _I64, _F32 = torch.int8, torch.int32, torch.int64, torch.float32
 _CODES = {torch.bfloat16: N.KL_DT_BF16, torch.float16: N.KL_DT_F16}
