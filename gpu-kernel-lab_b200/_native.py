@@ -155,20 +155,13 @@ _retired_workspaces: list = []
 
 
 def workspace(device: torch.device, nbytes: int, stream=None) -> torch.Tensor | None:
-    """``stream``: a ``torch.cuda.Stream`` of the device, or its raw handle (0: the default stream)."""
     if nbytes == 0:
         return None
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    if type(stream) is int and stream == 0:          # the default stream, which is never captured
-        buf = _workspaces.get(idx)
-        if buf is not None and buf.numel() >= nbytes:
-            return buf
     capturing = torch.cuda.is_current_stream_capturing()
     key = idx
-    if stream is not None and not capturing:
-        handle = stream if isinstance(stream, int) else stream.cuda_stream
-        if handle != 0:
-            key = (idx, handle)
+    if stream is not None and not capturing and stream != torch.cuda.default_stream(idx):
+        key = (idx, stream.cuda_stream)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
         if capturing:

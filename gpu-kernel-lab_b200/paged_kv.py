@@ -231,8 +231,9 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     * ``scale`` is ``head_dim ** -0.5`` if not given.
 
     Returns the output, or ``(output, lse)`` with ``return_lse``: f32 ``[batch, heads]``, the log of the sum of the
-    exponentials (``-inf`` for a length of 0), by which parts of a sequence can be joined.  ``workspace`` (uint8, zeroed
-    once, of ``paged_attention_workspace_bytes``) takes the place of the scratch kept per device and stream.
+    exponentials (``-inf`` for a length of 0), by which parts of a sequence can be joined.  ``workspace`` (uint8, of
+    ``paged_attention_workspace_bytes``) takes the place of scratch allocated for the call; calls that share one must not
+    overlap, on the device or, from several threads, on the host.
     """
     if _is_compiling():
         both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale)
@@ -269,8 +270,8 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     out = _empty(q, (batch, heads, dim), (heads * dim, dim, 1), dtype, index)
     lse = _empty(q, (batch, heads), (heads, 1), _F32, index) if return_lse else None
     if batch:
-        if workspace is None:
-            workspace = N.workspace(q.device, paged_attention_workspace_bytes(1, heads, kv_heads, dim), _raw_stream(index))
+        if workspace is None:                            # not N.workspace: another thread's call may come between this one's two launches
+            workspace = _empty(q, (paged_attention_workspace_bytes(1, heads, kv_heads, dim),), (1,), torch.uint8, index)
         elif workspace.get_device() != index or not workspace.is_contiguous():
             raise ValueError('workspace must be contiguous, on the cache\'s device')
         args = N.PAGED_ATTENTION_ARGS.pack(

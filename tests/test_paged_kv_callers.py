@@ -1,0 +1,72 @@
+"""How callers reach the operators of the paged key-value cache: from several threads, under torch's tracers, with a
+workspace of their own, with parameters, and with what is out of range.  Formulas and tolerances are
+``tests/test_paged_kv.py``'s."""
+import importlib.util
+import math
+import threading
+
+import pytest
+import torch
+
+from tests.conftest import ROOT
+from tests.test_paged_kv import LENGTHS, N, TYPES, attention, batch, check_attention, close, generator, kl, rope_tables, step_inputs
+
+gpu = pytest.mark.gpu
+P = kl.paged_kv
+WORKSPACE = 5                                                        # its place in PAGED_ATTENTION_ARGS
+
+
+def attend(case, **kw):
+    q, cache, table, lengths = case
+    return kl.paged_attention(q, cache.k_cache, cache.v_cache, table, lengths, cache.k_scales, cache.v_scales, **kw)
+
+
+# ---- scratch -------------------------------------------------------------------------
+@gpu
+def test_calls_under_way_have_scratch_of_their_own(monkeypatch):
+    """A call from another thread can come between the two launches of a split one: it must not have its scratch."""
+    cases = [batch(generator(i), torch.bfloat16, False, 4, 2, 128, 16, [3000, 50], poison=False) for i in (30, 31)]
+    refs = [attend(c) for c in cases]
+    real, seen = P._call, []
+
+    def call(index, fn, *args):
+        seen.append(N.PAGED_ATTENTION_ARGS.unpack(args[0])[WORKSPACE])
+        if len(seen) == 1:                                           # as another thread would, before this call launches
+            inner.append(attend(cases[1]))
+        real(index, fn, *args)
+
+    inner = []
+    monkeypatch.setattr(P, "_call", call)
+    outer = attend(cases[0])
+    assert seen[0] != seen[1]
+    assert torch.equal(outer, refs[0]) and torch.equal(inner[0], refs[1])
+
+
+@gpu
+def test_threads_on_one_stream():
+    """Rows at other places of outputs of other sizes, from threads that share the default stream, linears between them."""
+    w = kl.quantize_int8_rowwise(torch.randn(512, 512, generator=generator(2), device="cuda"))
+    x = torch.randn(4, 512, generator=generator(3), device="cuda").bfloat16()
+    cases = [batch(generator(40 + i), torch.bfloat16, False, 4, 2, 128, 16, lengths, poison=False)
+             for i, lengths in enumerate(([4000], [70, 3000, 900], [2500] * 5, [5, 5000]))]
+    refs = [attend(c) for c in cases]
+    torch.cuda.synchronize()
+    outs, failed, start = [[] for _ in cases], [], threading.Barrier(len(cases))
+
+    def work(i):
+        try:
+            start.wait()
+            for _ in range(60):
+                outs[i].append(attend(cases[i]))
+                kl.quant_linear(x, w)
+        except Exception as e:                                       # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for out, ref in zip(outs, refs):
+        assert len(out) == 60 and all(torch.equal(o, ref) for o in out)
