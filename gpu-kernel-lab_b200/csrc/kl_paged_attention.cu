@@ -33,8 +33,8 @@
 // Scores, softmax statistics and the output are f32; the reference of the
 // exponentials is not the running maximum but follows it only when a score
 // exceeds it by 2^8, which spares a reduction over the keys at nearly every unit. The weights P
-// enter the second product as two 16-bit numbers p = hi + lo (16 bits of bf16 or 22
-// of f16), so that their rounding stays below the output's. With up to four
+// enter the second product as two 16-bit numbers p = hi + lo (16 bits of bf16; f16: at kF16Lift),
+// so that their rounding stays below the output's. With up to four
 // heads per KV head the heads stand twice in the eight columns and the second
 // copy carries lo: no product more (2 % faster for int8, even for bf16). Int8
 // keys and values are converted exactly, five operations per four of them (to
@@ -71,7 +71,13 @@ constexpr int kWholeUnits = 4;
 // among short ones can cost.
 constexpr int kWholeUnitsOfMany = 16;
 constexpr int kMaxLens = 512;          // lengths kept in shared memory
-constexpr float kSlack = 8.0f;           // log2 of how far weights may exceed 1
+constexpr float kSlack = 8.0f;           // log2 of how far the largest weight of a key may grow before the reference moves
+// f16 has 40 binades. Weights of f16 values use them all: the largest is between 2^7 and 2^15 (the reference is 2^7 below
+// the largest score), and the low parts are carried times 2^12 and summed apart. A weight then has 22 bits down to 2^-20 of the
+// largest and an error of at most 2^-44 of it below. With weights from 1 and both parts in one sum the step of f16's subnormals
+// left 12 bits at 2^-13 and none at 2^-25, which the sum of the weights still counted: thousands of keys behind one of
+// a large weight came out 4 % low at 2^-21. Bf16 has the exponents of f32 and needs neither.
+constexpr float kF16Lift = 7.0f, kF16Low = 4096.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -234,6 +240,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr bool kQkBf16 = kBf16;                   // type of the K Q^T product
   constexpr bool kPvBf16 = kBf16 || INT8;           // type of the V^T P^T product
+  constexpr float kLift = kPvBf16 ? 0.0f : kF16Lift;
   constexpr int kChunks = G::kRow / 16;             // 16-byte chunks of one key
   constexpr int kRowsPer = 32 / kChunks;            // keys that one warp-wide copy covers
   constexpr int kWords = (G::kKeys + 31) / 32;      // keys per lane
@@ -597,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
         }
       }
     }
-    // scores; the reference of the exponentials moves only when one exceeds it by 2^8
+    // scores; the reference of the exponentials moves only when one exceeds it by 2^(kLift + 8)
     bool above = false;
 #pragma unroll
     for (int g = 0; g < G::kTiles; ++g) {
@@ -630,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
         most[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
         for (int g = 1; g < G::kTiles; ++g) most[nt][e] = fmaxf(most[nt][e], fmaxf(s[g][nt][e], s[g][nt][2 + e]));
-        above |= most[nt][e] > top[nt][e] + kSlack;
+        above |= most[nt][e] > top[nt][e] + (kLift + kSlack);
       }
     if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
@@ -638,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(most[nt][e], top[nt][e]);
+          float x = fmaxf(most[nt][e] - kLift, top[nt][e]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
           f[e] = ex2(top[nt][e] - x);
@@ -686,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
           const float p0 = s[g][nt][2 * h], p1 = s[g][nt][2 * h + 1];
           uint32_t w = pack2<kPvBf16>(p0, p1);
           const float2 f = unpack2<kPvBf16>(w);
-          const uint32_t rest = pack2<kPvBf16>(p0 - f.x, p1 - f.y);
+          const uint32_t rest = kPvBf16 ? pack2<kPvBf16>(p0 - f.x, p1 - f.y) : pack2<kPvBf16>((p0 - f.x) * kF16Low, (p1 - f.y) * kF16Low);
           if constexpr (G::kDup) {
             hi[nt][h] = movmatrix_t(t4 < 2 ? w : rest);
           } else {
@@ -720,7 +727,13 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
 #pragma unroll
           for (int nt = 0; nt < G::kNT; ++nt) {
             mma16816<kPvBf16>(acc[m][nt], r[0], r[1], r[2], r[3], hi[nt][0], hi[nt][1]);
-            if constexpr (!G::kDup) mma16816<kPvBf16>(acc[m][nt], r[0], r[1], r[2], r[3], lo[nt][0], lo[nt][1]);
+            if constexpr (!G::kDup && kPvBf16) mma16816<kPvBf16>(acc[m][nt], r[0], r[1], r[2], r[3], lo[nt][0], lo[nt][1]);
+            if constexpr (!G::kDup && !kPvBf16) {
+              float low[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma16816<kPvBf16>(low, r[0], r[1], r[2], r[3], lo[nt][0], lo[nt][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][nt][e] = fmaf(low[e], 1.0f / kF16Low, acc[m][nt][e]);
+            }
           }
         }
       }
@@ -735,6 +748,8 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     const int first = at.head * a.group + at.block * HB, n = min(HB, a.group - at.block * HB);
     __syncwarp();
     float* o = out_slot(warp, slot);
+    // codes entered as q / 64; the second copy of the heads holds the low parts
+    const float unit = INT8 ? 64.0f : !kPvBf16 && G::kDup && t4 >= 2 ? 1.0f / kF16Low : 1.0f;
 #pragma unroll
     for (int nt = 0; nt < G::kNT; ++nt)
 #pragma unroll
@@ -751,8 +766,8 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
 #pragma unroll
           for (int m = 0; m < D / 16; ++m) {
             const int d0 = INT8 ? m * 16 + 2 * l4 : m * 16 + l4, d1 = INT8 ? d0 + 1 : d0 + 8;
-            o[spread(col, d0)] = INT8 ? acc[m][nt][e] * 64.0f : acc[m][nt][e];
-            o[spread(col, d1)] = INT8 ? acc[m][nt][2 + e] * 64.0f : acc[m][nt][2 + e];
+            o[spread(col, d0)] = acc[m][nt][e] * unit;
+            o[spread(col, d1)] = acc[m][nt][2 + e] * unit;
           }
         }
       }

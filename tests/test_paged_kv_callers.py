@@ -70,3 +70,21 @@ def test_threads_on_one_stream():
     assert not failed
     for out, ref in zip(outs, refs):
         assert len(out) == 60 and all(torch.equal(o, ref) for o in out)
+
+
+# ---- weights of f16 caches --------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (8, 8, 64), (16, 2, 128), (8, 1, 64), (32, 2, 128), (16, 1, 64), (12, 1, 256)])
+@pytest.mark.parametrize("low,high", [(-28.0, -16.0), (-20.62, -20.62), (-25.5, -25.5)])
+def test_small_weights_of_f16_caches(heads, kv_heads, dim, low, high):
+    """One key in eight has nearly all the weight and values of zero; the output is that of the others, 2^low to 2^high of it."""
+    g = generator(dim + heads)
+    q, cache, table, lengths = batch(g, torch.float16, False, heads, kv_heads, dim, 16, [4097, 300, 16385, 17], poison=False)
+    q.zero_()
+    q[..., 0] = 1.0
+    k = low + (high - low) * torch.rand(cache.k_cache.shape[:3], generator=g, device="cuda")
+    heavy = torch.rand(k.shape, generator=g, device="cuda") < 0.125
+    cache.k_cache[..., 0] = torch.where(heavy, 0.0, k)
+    cache.v_cache.copy_(500 + 1000 * torch.rand(cache.v_cache.shape, generator=g, device="cuda"))
+    cache.v_cache[heavy] = 0.0
+    check_attention(q, cache, table, lengths, scale=math.log(2.0))
