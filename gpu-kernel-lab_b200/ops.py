@@ -201,19 +201,19 @@ _lib.define("read_kv(Tensor k_cache, Tensor v_cache, Tensor slots, Tensor? k_sca
             "ScalarType? dtype=None) -> (Tensor, Tensor)")
 
 
-def _paged_attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None):
+def _paged_attention_cuda(*args, **kwargs):
     from . import paged_kv
-    return paged_kv.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, return_lse=True)
+    return paged_kv.attention_cuda(*args, **kwargs)
 
 
 def _qk_norm_rope_write_cuda(*args, **kwargs):
     from . import paged_kv
-    return paged_kv.qk_norm_rope_write(*args, **kwargs)
+    return paged_kv.write_cuda(*args, **kwargs)
 
 
 def _read_kv_cuda(*args, **kwargs):
     from . import paged_kv
-    return paged_kv.read_kv(*args, **kwargs)
+    return paged_kv.read_cuda(*args, **kwargs)
 
 
 _lib.impl("paged_attention", _paged_attention_cuda, "CUDA")

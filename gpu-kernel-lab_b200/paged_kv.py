@@ -23,8 +23,10 @@ Arguments are checked on the host (``ValueError``).  What only the device sees
 outside the buffers and is recorded for ``_native.device_status``.
 
 The functions are for inference: tensors that require grad are refused, as
-``qwen_rmsnorm`` refuses them.  Called eagerly they launch directly; where torch
-traces them they are the operators ``torch.ops.kl_b200.*`` of the same names.
+``qwen_rmsnorm`` refuses them.  Called eagerly they launch directly; under
+``torch.compile``, ``torch.export``, ``make_fx``, ``torch.jit.trace``, a fake or other dispatch mode, a
+``torch.func`` transform or with tensors of a subclass they are the operators
+``torch.ops.kl_b200.*`` of the same names.
 """
 from __future__ import annotations
 
@@ -44,6 +46,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 _empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 _is_compiling = torch.compiler.is_compiling
+# Who may be looking at a call: dispatch modes (make_fx, fake tensors), jit.trace, torch.func. A torch that lacks one of these
+# names takes every call through the operators.
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_tracing = getattr(torch._C, "_is_tracing", None)
+_transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", None)
+_BLIND = None in (_modes, _tracing, _transform)
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 _I8, _I32, _I64, _F32 = torch.int8, torch.int32, torch.int64, torch.float32
 _CODES = {torch.bfloat16: N.KL_DT_BF16, torch.float16: N.KL_DT_F16}
 
@@ -73,6 +82,12 @@ def new_kv_cache(pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, dev
 def kv_slots(page_table, rows, positions, page_size):
     """Slots (int64) of ``positions`` of the sequences ``rows`` of ``page_table``."""
     return page_table[rows, positions // page_size].long() * page_size + positions % page_size
+
+
+def _traced(x, cache):
+    """Whether a call is to go through the dispatcher: its outputs are allocated past it otherwise, and unknown to who traces it."""
+    return (_is_compiling() or _BLIND or _modes() > 0 or _tracing() or _transform() is not None
+            or type(x) not in _PLAIN or type(cache) not in _PLAIN)
 
 
 def _pack_cache(k_cache, v_cache, k_scales, v_scales, dtype, index):
@@ -151,9 +166,12 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
 
     The arithmetic is f32 up to one rounding at the store (an int8 cache quantises the f32 value).
     """
-    if _is_compiling():
-        return torch.ops.kl_b200.qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache,
-                                                    k_scales, v_scales, epsilon)
+    call = torch.ops.kl_b200.qk_norm_rope_write if _traced(q, k_cache) else write_cuda
+    return call(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales, v_scales, epsilon)
+
+
+def write_cuda(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales=None, v_scales=None, epsilon=1e-6):
+    """``qk_norm_rope_write`` on CUDA tensors."""
     shape, kv_shape = q.shape, k.shape
     if len(shape) != 3 or len(kv_shape) != 3 or v.shape != kv_shape or shape[0] != kv_shape[0] or shape[2] != kv_shape[2]:
         raise ValueError('q must be [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]')
@@ -202,8 +220,12 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
 
     ``dtype`` (bf16 or f16) is that of the result of an int8 cache, bf16 if not given; a 16-bit cache returns its own.
     """
-    if _is_compiling():
-        return torch.ops.kl_b200.read_kv(k_cache, v_cache, slots, k_scales, v_scales, dtype)
+    call = torch.ops.kl_b200.read_kv if _traced(slots, k_cache) else read_cuda
+    return call(k_cache, v_cache, slots, k_scales, v_scales, dtype)
+
+
+def read_cuda(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
+    """``read_kv`` on CUDA tensors."""
     if dtype is None:
         dtype = torch.bfloat16 if k_cache.dtype is _I8 else k_cache.dtype
     if dtype not in _CODES:
@@ -235,9 +257,15 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     ``paged_attention_workspace_bytes``) takes the place of scratch allocated for the call; calls that share one must not
     overlap, on the device or, from several threads, on the host.
     """
-    if _is_compiling():
+    if _traced(q, k_cache):
         both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale)
         return both if return_lse else both[0]
+    return attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, return_lse, workspace)
+
+
+def attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None, return_lse=True,
+                   workspace=None):
+    """``paged_attention`` on CUDA tensors."""
     shape = q.shape
     if len(shape) != 3:
         raise ValueError('q must be [batch, heads, head_dim]')

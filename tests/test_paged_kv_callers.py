@@ -88,3 +88,79 @@ def test_small_weights_of_f16_caches(heads, kv_heads, dim, low, high):
     cache.v_cache.copy_(500 + 1000 * torch.rand(cache.v_cache.shape, generator=g, device="cuda"))
     cache.v_cache[heavy] = 0.0
     check_attention(q, cache, table, lengths, scale=math.log(2.0))
+
+
+# ---- tracers -----------------------------------------------------------------------------
+def fake_step():
+    """Shapes of a step, for a fake mode."""
+    q, k = (torch.empty(5, h, 128, dtype=torch.bfloat16, device="cuda") for h in (4, 2))
+    cache = torch.empty(3, 2, 16, 128, dtype=torch.bfloat16, device="cuda")
+    at, cos = torch.empty(5, dtype=torch.int64, device="cuda"), torch.empty(9, 64, device="cuda")
+    return q, k, cache, at, cos, torch.empty(5, 3, dtype=torch.int32, device="cuda"), torch.empty(5, dtype=torch.int32, device="cuda")
+
+
+def all_three(q, k, cache, at, cos, table, lengths):
+    turned = kl.qk_norm_rope_write(q, k, k, None, None, cos, cos, at, at, cache, cache)
+    return kl.paged_attention(turned, cache, cache, table, lengths), *kl.read_kv(cache, cache, at)
+
+
+def test_functions_give_shapes_under_a_fake_mode():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        args = fake_step()
+        out, k, v = all_three(*args)
+    assert out.shape == (5, 4, 128) and k.shape == v.shape == (5, 2, 128) and out.dtype == torch.bfloat16
+    out, k, v = all_three(*args)                                     # fake tensors after their mode
+    assert out.shape == (5, 4, 128) and k.shape == v.shape == (5, 2, 128)
+
+
+@pytest.mark.parametrize("mode", ["real", "symbolic"])
+def test_functions_are_operators_in_a_traced_graph(mode):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.fx.experimental.symbolic_shapes import ShapeEnv
+    if mode == "real":                                               # traced as they are: tensors that are fake before
+        with FakeTensorMode():
+            graph = make_fx(all_three)(*fake_step())
+    else:
+        with FakeTensorMode(shape_env=ShapeEnv()):
+            args = fake_step()
+        graph = make_fx(all_three, tracing_mode="symbolic")(*args)
+    names = [str(n.target) for n in graph.graph.nodes]
+    for name in ("qk_norm_rope_write", "paged_attention", "read_kv"):
+        assert sum(name in n for n in names) == 1
+
+
+@gpu
+@pytest.mark.parametrize("tracer", ["make_fx", "jit", "functionalize"])
+def test_traced_calls_follow_their_inputs(tracer):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    cases = [batch(generator(50 + i), torch.bfloat16, True, 4, 2, 128, 16, [700, 40, 9], poison=False) for i in range(2)]
+    cos, sin = rope_tables(None, 128, 1000)
+
+    def step(q, k, c, d, cs, ds, table, lengths, positions, slots):
+        if tracer != "functionalize":                                # which takes no operator that writes to its arguments
+            q = kl.qk_norm_rope_write(q, k, k * 2, None, None, cos, sin, positions, slots, c, d, cs, ds)
+        out, lse = kl.paged_attention(q, c, d, table, lengths, cs, ds, return_lse=True)
+        k, v = kl.read_kv(c, d, slots, cs, ds)
+        return out, lse, k, v
+
+    inputs = []
+    for i, (q, cache, table, lengths) in enumerate(cases):
+        k = torch.randn(3, 2, 128, generator=generator(60 + i), device="cuda").bfloat16()
+        at = lengths.long() - 1
+        inputs.append((q, k, *cache, table, lengths, at, kl.kv_slots(table, torch.arange(3, device="cuda"), at, 16)))
+
+    def copies(args):
+        return [t.clone() for t in args]
+
+    refs = [step(*copies(args)) for args in inputs]
+    if tracer == "functionalize":
+        traced = make_fx(torch.func.functionalize(step))(*copies(inputs[0]))
+    elif tracer == "make_fx":
+        traced = make_fx(step)(*copies(inputs[0]))
+    else:
+        traced = torch.jit.trace(step, tuple(copies(inputs[0])), check_trace=False)
+    for args, ref in zip(inputs, refs):
+        got = traced(*copies(args))
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
