@@ -193,7 +193,7 @@ def _int4_head_fake(x, data, scales, group, top_k, block_n):
 
 # ---- paged key-value cache ----------------------------------------------------------
 _lib.define("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor page_table, Tensor lengths, "
-            "Tensor? k_scales=None, Tensor? v_scales=None, float? scale=None) -> (Tensor, Tensor)")
+            "Tensor? k_scales=None, Tensor? v_scales=None, float? scale=None, Tensor? workspace=None) -> (Tensor, Tensor)")
 _lib.define("qk_norm_rope_write(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, "
             "Tensor positions, Tensor slots, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scales=None, "
             "Tensor(d!)? v_scales=None, float epsilon=1e-6) -> Tensor")
@@ -222,7 +222,7 @@ _lib.impl("read_kv", _read_kv_cuda, "CUDA")
 
 
 @torch.library.register_fake("kl_b200::paged_attention")
-def _paged_attention_fake(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None):
+def _paged_attention_fake(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None, workspace=None):
     return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
 
 

@@ -258,13 +258,13 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     overlap, on the device or, from several threads, on the host.
     """
     if _traced(q, k_cache):
-        both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale)
+        both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, workspace)
         return both if return_lse else both[0]
-    return attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, return_lse, workspace)
+    return attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, workspace, return_lse)
 
 
-def attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None, return_lse=True,
-                   workspace=None):
+def attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_scales=None, scale=None, workspace=None,
+                   return_lse=True):
     """``paged_attention`` on CUDA tensors."""
     shape = q.shape
     if len(shape) != 3:

@@ -164,3 +164,32 @@ def test_traced_calls_follow_their_inputs(tracer):
     for args, ref in zip(inputs, refs):
         got = traced(*copies(args))
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_a_traced_call_keeps_its_workspace():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with FakeTensorMode():
+        q, _, cache, _, _, table, lengths = fake_step()
+        space = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+        graph = make_fx(lambda q, space: kl.paged_attention(q, cache, cache, table, lengths, workspace=space))(q, space)
+    call, = (n for n in graph.graph.nodes if "paged_attention" in str(n.target))
+    given = [n for n in graph.graph.nodes if n.op == "placeholder"]
+    assert given[1] in call.all_input_nodes
+
+
+@gpu
+def test_a_compiled_call_uses_its_workspace(monkeypatch):
+    case = batch(generator(33), torch.bfloat16, False, 4, 2, 128, 16, [3000, 50], poison=False)
+    space = torch.zeros(kl.paged_attention_workspace_bytes(2, 4, 2, 128), dtype=torch.uint8, device="cuda")
+    ref, real, seen = attend(case), P._call, []
+
+    def call(index, fn, *args):
+        seen.append(N.PAGED_ATTENTION_ARGS.unpack(args[0])[WORKSPACE])
+        real(index, fn, *args)
+
+    compiled = torch.compile(lambda space: attend(case, workspace=space), backend="aot_eager", fullgraph=True)
+    monkeypatch.setattr(P, "_call", call)
+    assert torch.equal(compiled(space), ref) and seen == [space.data_ptr()]
+    with pytest.raises(Exception, match="workspace"):
+        compiled(space[:64])
