@@ -33,6 +33,7 @@ EXPORTED_SYMBOLS = (
     "kl_linear_noalloc", "kl_topk_rows_workspace_bytes", "kl_topk_rows", "kl_topk_merge_rows", "kl_rmsnorm",
     "kl_linear_topk", "kl_linear_topk_workspace_bytes", "kl_grouped_digits_bytes", "kl_grouped_encode_ex",
     "kl_qk_norm_rope_write", "kl_read_kv", "kl_paged_attention", "kl_paged_attention_workspace_bytes",
+    "kl_paged_attention_call_bytes",
 )
 
 
@@ -82,6 +83,7 @@ _SIGNATURES = {
     "kl_read_kv": (_I, [_P, _I, _P, _I, _P, _P, _P]),
     "kl_paged_attention": (_I, [_P, _P]),
     "kl_paged_attention_workspace_bytes": (_S, [_I, _I, _I, _I]),
+    "kl_paged_attention_call_bytes": (_S, [_I, _I, _I, _I, _I, _I, _I]),
 }
 
 _lib = None

@@ -955,6 +955,11 @@ size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, in
   return paged_attention_workspace_bytes(heads, kv_heads, head_dim, sm_count_or_default());
 }
 
+size_t kl_paged_attention_call_bytes(int batch, int heads, int kv_heads, int head_dim, int format, int columns, int page_size) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || columns < 0 || page_size <= 0) return 0;
+  return paged_attention_call_bytes(batch, heads, kv_heads, head_dim, format == KL_KV_INT8, columns, page_size, sm_count_or_default());
+}
+
 int kl_paged_attention(const kl_paged_attention_args* args, void* stream) {
   if (!args) return fail(KL_ERR_INVALID, "args must be non-null");
   const kl_paged_attention_args& a = *args;
@@ -976,8 +981,8 @@ int kl_paged_attention(const kl_paged_attention_args* args, void* stream) {
     return fail(KL_ERR_INVALID, "batch * heads * (columns * page_size / 64 + 1) must stay below 2^31");
   DeviceInfo di;
   if ((rc = check_device(&di)) != KL_OK) return rc;
-  const size_t need = paged_attention_workspace_bytes(a.heads, c.kv_heads, c.head_dim, di.sm_count);
-  if (!a.workspace || a.workspace_bytes < need)
+  const size_t need = paged_attention_call_bytes(a.batch, a.heads, c.kv_heads, c.head_dim, c.format == KL_KV_INT8, a.columns, c.page_size, di.sm_count);
+  if (need && (!a.workspace || a.workspace_bytes < need))
     return fail(KL_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, a.workspace ? a.workspace_bytes : 0);
   if (!aligned16(a.workspace)) return fail(KL_ERR_INVALID, "workspace must be 16-byte aligned");
   const cudaError_t e = launch_paged_attention(a, di.sm_count, di.status, static_cast<cudaStream_t>(stream));

@@ -255,6 +255,7 @@ cudaError_t launch_kv_read(const kl_kv_cache& cache, int dtype, const int64_t* s
 void* tensor_map_encoder();
 // kl_paged_attention.cu
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int sm_count);
+size_t paged_attention_call_bytes(int batch, int heads, int kv_heads, int head_dim, bool int8, int columns, int page_size, int sm_count);
 cudaError_t launch_paged_attention(const kl_paged_attention_args& args, int sm_count, int* status, cudaStream_t s);
 
 // ---------------------------------------------------------- quantisation

@@ -946,6 +946,18 @@ int make_maps(const AttnArgs& a, AttnMaps<INT8>& maps, int head_dim, int span, i
   return box;
 }
 
+// How a call is dealt out: by what is known before the lengths are
+struct Deal {
+  bool whole;                          // rows are not split
+  unsigned grid;
+};
+template <typename G>
+Deal deal(long long rows, long long room, int sm_count) {
+  const long long most = rows * ((room + G::kUnit - 1) / G::kUnit), wave = static_cast<long long>(sm_count) * G::kResident;
+  return {room <= (rows >= 2 * wave ? kWholeUnitsOfMany : kWholeUnits) * G::kUnit,
+          static_cast<unsigned>(std::max(1ll, std::min({most, wave, static_cast<long long>(kMaxCtas)})))};
+}
+
 template <typename T, bool INT8, int D, int HB>
 cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
   using G = Geo<INT8, D, HB>;
@@ -961,14 +973,11 @@ cudaError_t attn_hb(AttnArgs& a, int sm_count, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     allowed.fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
-  const long long room = static_cast<long long>(a.columns) * a.kv.page_size;
-  const long long rows = static_cast<long long>(a.batch) * a.kv.kv_heads * a.blocks, most = rows * ((room + G::kUnit - 1) / G::kUnit);
-  const long long wave = static_cast<long long>(sm_count) * G::kResident;
-  const bool whole = room <= (rows >= 2 * wave ? kWholeUnitsOfMany : kWholeUnits) * G::kUnit;
-  const unsigned grid = static_cast<unsigned>(std::max(1ll, std::min({most, wave, static_cast<long long>(kMaxCtas)})));
-  char* const space = static_cast<char*>(a.workspace) + kCounterBytes;
+  const auto [whole, grid] =
+      deal<G>(static_cast<long long>(a.batch) * a.kv.kv_heads * a.blocks, static_cast<long long>(a.columns) * a.kv.page_size, sm_count);
+  char* const space = whole ? nullptr : static_cast<char*>(a.workspace) + kCounterBytes;
   a.records = whole ? nullptr : reinterpret_cast<Piece*>(space);
-  a.partials = reinterpret_cast<float*>(space + kRecordBytes);
+  a.partials = whole ? nullptr : reinterpret_cast<float*>(space + kRecordBytes);
   e = launch_dependent(attn_kernel<T, INT8, D, HB>, dim3(grid), kThreads, G::kSmem, s, a, maps);
   if (e != cudaSuccess || !a.records) return e;
   const unsigned parts = (std::min(a.group, HB) + join_heads(HB) - 1) / join_heads(HB);
@@ -998,10 +1007,32 @@ cudaError_t attn_t(AttnArgs& a, int head_dim, int sm_count, cudaStream_t s) {
 
 }  // namespace
 
+// The records, and two partial rows per CTA
+size_t bytes_for(unsigned ctas, int hb, int head_dim) {
+  return kCounterBytes + kRecordBytes + 2ull * ctas * hb * (head_dim + 2) * sizeof(float);
+}
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int sm_count) {
-  // the records, and two partial rows per CTA of the widest wave
-  const int hb = heads_per_cta(heads / std::max(1, kv_heads), head_dim);
-  return kCounterBytes + kRecordBytes + 2ull * std::min(3 * sm_count, kMaxCtas) * hb * (head_dim + 2) * sizeof(float);
+  return bytes_for(std::min(3 * sm_count, kMaxCtas), heads_per_cta(heads / std::max(1, kv_heads), head_dim), head_dim);
+}
+
+template <bool INT8, int D>
+Deal deal_of(int hb, long long rows, long long room, int sm_count) {
+  if (hb == 4) return deal<Geo<INT8, D, 4>>(rows, room, sm_count);
+  if constexpr (D != 256)
+    if (hb == 16) return deal<Geo<INT8, D, 16>>(rows, room, sm_count);
+  return deal<Geo<INT8, D, 8>>(rows, room, sm_count);
+}
+template <bool INT8>
+Deal deal_of(int hb, int head_dim, long long rows, long long room, int sm_count) {
+  return head_dim == 64    ? deal_of<INT8, 64>(hb, rows, room, sm_count)
+         : head_dim == 128 ? deal_of<INT8, 128>(hb, rows, room, sm_count)
+                           : deal_of<INT8, 256>(hb, rows, room, sm_count);
+}
+size_t paged_attention_call_bytes(int batch, int heads, int kv_heads, int head_dim, bool int8, int columns, int page_size, int sm_count) {
+  const int group = heads / kv_heads, hb = heads_per_cta(group, head_dim);
+  const long long rows = static_cast<long long>(batch) * kv_heads * ((group + hb - 1) / hb), room = static_cast<long long>(columns) * page_size;
+  const Deal d = int8 ? deal_of<true>(hb, head_dim, rows, room, sm_count) : deal_of<false>(hb, head_dim, rows, room, sm_count);
+  return d.whole ? 0 : bytes_for(d.grid, hb, head_dim);
 }
 
 cudaError_t launch_paged_attention(const kl_paged_attention_args& p, int sm_count, int* status, cudaStream_t s) {
@@ -1024,7 +1055,7 @@ cudaError_t launch_paged_attention(const kl_paged_attention_args& p, int sm_coun
   a.scale = p.scale;
   a.out = p.out;
   a.lse = p.lse;
-  a.workspace = p.workspace;
+  a.workspace = p.workspace;                        // may be null where rows are not split
   a.status = status;
   const bool int8 = p.cache.format == KL_KV_INT8;
   if (p.dtype == KL_DT_BF16)

@@ -154,6 +154,13 @@ def paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim) -> int:
     return N.lib().kl_paged_attention_workspace_bytes(batch, heads, kv_heads, head_dim)
 
 
+@functools.lru_cache(maxsize=1024)
+def _call_bytes(batch, heads, kv_heads, head_dim, quantized, columns, page_size) -> int:
+    """Of that scratch, what one call needs: nothing where its rows are not split."""
+    return N.lib().kl_paged_attention_call_bytes(batch, heads, kv_heads, head_dim, N.KL_KV_INT8 if quantized else N.KL_KV_SAME, columns,
+                                                 page_size)
+
+
 def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales=None, v_scales=None,
                        epsilon=1e-6):
     """Normalise and rotate queries and keys, write keys and values to ``slots``; returns the queries.
@@ -299,12 +306,13 @@ def attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_sc
     lse = _empty(q, (batch, heads), (heads, 1), _F32, index) if return_lse else None
     if batch:
         if workspace is None:                            # not N.workspace: another thread's call may come between this one's two launches
-            workspace = _empty(q, (paged_attention_workspace_bytes(1, heads, kv_heads, dim),), (1,), torch.uint8, index)
+            need = _call_bytes(batch, heads, kv_heads, dim, k_cache.dtype is _I8, table[1], k_cache.shape[2])
+            workspace = _empty(q, (need,), (1,), torch.uint8, index) if need else None
         elif workspace.get_device() != index or not workspace.is_contiguous():
             raise ValueError('workspace must be contiguous, on the cache\'s device')
         args = N.PAGED_ATTENTION_ARGS.pack(
             q.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            workspace.data_ptr(), workspace.nbytes, strides[0], strides[1], table_stride, cache, _CODES[dtype], batch, heads, table[1],
-            scale)
+            0 if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.nbytes, strides[0], strides[1],
+            table_stride, cache, _CODES[dtype], batch, heads, table[1], scale)
         _call(index, N.lib().kl_paged_attention, args)
     return (out, lse) if return_lse else out

@@ -373,11 +373,14 @@ int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int to
  *   past a sequence's length are not read.  A length beyond columns *
  *   page_size is cut to it, and keys of a page id out of range count
  *   as absent; both record KL_ERR_INVALID in the device status word.
- *   workspace: kl_paged_attention_workspace_bytes(...) bytes, 16-byte aligned.
+ *   workspace: kl_paged_attention_workspace_bytes(...) bytes serve any call of these heads;
+ *   kl_paged_attention_call_bytes(...) are what one call needs, 0 (NULL allowed) where its rows
+ *   are not split. 16-byte aligned.
  *   It may be kl_linear's: the first 64 KiB, which that needs zeroed, are left as
  *   they are.  Calls that share a workspace must not run concurrently.
  */
 size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim);
+size_t kl_paged_attention_call_bytes(int batch, int heads, int kv_heads, int head_dim, int format, int columns, int page_size);
 typedef struct kl_paged_attention_args {
   const void* q;
   const int32_t* page_table;

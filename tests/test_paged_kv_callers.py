@@ -72,6 +72,19 @@ def test_threads_on_one_stream():
         assert len(out) == 60 and all(torch.equal(o, ref) for o in out)
 
 
+def test_scratch_of_one_call():
+    """None for rows that are not split, and never more than what serves any call of these heads."""
+    bytes_for = N.lib().kl_paged_attention_call_bytes
+    for heads, kv_heads, dim in ((4, 2, 128), (8, 8, 64), (16, 2, 128), (32, 2, 128), (40, 1, 64), (12, 1, 256)):
+        for form in (N.KL_KV_SAME, N.KL_KV_INT8):
+            assert bytes_for(1, heads, kv_heads, dim, form, 0, 16) == bytes_for(3, heads, kv_heads, dim, form, 16, 16) == 0
+            assert bytes_for(2000, heads, kv_heads, dim, form, 1000, 1) == 0
+            most = kl.paged_attention_workspace_bytes(1, heads, kv_heads, dim)
+            sizes = [bytes_for(b, heads, kv_heads, dim, form, columns, 16) for b in (1, 3) for columns in (100, 5000)]
+            assert all(0 < n <= most for n in sizes) and max(sizes) > sizes[0]
+    assert bytes_for(0, 4, 2, 128, N.KL_KV_SAME, 100, 16) == 0
+
+
 # ---- weights of f16 caches --------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 128), (8, 8, 64), (16, 2, 128), (8, 1, 64), (32, 2, 128), (16, 1, 64), (12, 1, 256)])
