@@ -80,8 +80,19 @@ def new_kv_cache(pages, page_size, kv_heads, head_dim, dtype=torch.bfloat16, dev
 
 
 def kv_slots(page_table, rows, positions, page_size):
-    """Slots (int64) of ``positions`` of the sequences ``rows`` of ``page_table``."""
-    return page_table[rows, positions // page_size].long() * page_size + positions % page_size
+    """Slots (int64) of ``positions`` of the sequences ``rows`` of ``page_table``.
+
+    A position that the table has no column for has slot -1, which is not cached: one before the sequence, as ``lengths - 1`` of an
+    empty one is, or past its pages.
+    """
+    columns = page_table.shape[1]
+    if columns == 0:
+        return torch.full_like(positions + rows, -1, dtype=torch.int64)
+    positions = positions.long()
+    column = positions // page_size
+    there = column.clamp(0, columns - 1)
+    slots = torch.add(positions % page_size, page_table[rows, there], alpha=page_size)
+    return torch.where(column == there, slots, -1)
 
 
 def _traced(x, cache):

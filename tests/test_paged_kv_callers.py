@@ -206,3 +206,19 @@ def test_a_compiled_call_uses_its_workspace(monkeypatch):
     assert torch.equal(compiled(space), ref) and seen == [space.data_ptr()]
     with pytest.raises(Exception, match="workspace"):
         compiled(space[:64])
+
+
+# ---- positions and arguments ----------------------------------------------------------------
+def test_kv_slots_of_positions_outside_the_table():
+    """A position before the sequence or past its pages has no slot: negative, so not cached."""
+    table = torch.tensor([[4, 2], [0, 9]], dtype=torch.int32)
+    for kind in (torch.int32, torch.int64):
+        rows, positions = torch.tensor([0, 0, 1, 1, 0, 1]), torch.tensor([-1, 17, -16, 32, 2 ** 30, 31], dtype=kind)
+        slots = kl.kv_slots(table, rows, positions, 16)
+        assert slots.dtype == torch.int64 and slots[[1, 5]].tolist() == [33, 9 * 16 + 15]
+        assert (slots[[0, 2, 3, 4]] < 0).all()
+    unused = torch.tensor([[7, -1]], dtype=torch.int32)              # a column that is not used yet
+    assert (kl.kv_slots(unused, torch.zeros(16, dtype=torch.int64), torch.arange(16, 32), 16) < 0).all()
+    none = torch.zeros(2, 0, dtype=torch.int32)
+    assert (kl.kv_slots(none, torch.tensor([0, 1]), torch.tensor([0, 5]), 16) < 0).all()
+    assert kl.kv_slots(none, torch.tensor([], dtype=torch.int64), torch.tensor([], dtype=torch.int64), 16).shape == (0,)
