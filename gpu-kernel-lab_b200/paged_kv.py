@@ -45,7 +45,7 @@ HEAD_DIMS = (64, 128, 256)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 _empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
-_is_compiling = torch.compiler.is_compiling
+_is_compiling, _is_grad_enabled = torch.compiler.is_compiling, torch.is_grad_enabled
 # Who may be looking at a call: dispatch modes (make_fx, fake tensors), jit.trace, torch.func. A torch that lacks one of these
 # names takes every call through the operators.
 _modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
@@ -93,6 +93,13 @@ def kv_slots(page_table, rows, positions, page_size):
     there = column.clamp(0, columns - 1)
     slots = torch.add(positions % page_size, page_table[rows, there], alpha=page_size)
     return torch.where(column == there, slots, -1)
+
+
+def _refuse_grad(*tensors):
+    if _is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError('inference only; use torch.inference_mode()')
 
 
 def _traced(x, cache):
@@ -184,6 +191,7 @@ def qk_norm_rope_write(q, k, v, q_weight, k_weight, cos, sin, positions, slots, 
 
     The arithmetic is f32 up to one rounding at the store (an int8 cache quantises the f32 value).
     """
+    _refuse_grad(q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache, k_scales, v_scales)
     call = torch.ops.kl_b200.qk_norm_rope_write if _traced(q, k_cache) else write_cuda
     return call(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache, k_scales, v_scales, epsilon)
 
@@ -222,8 +230,6 @@ def write_cuda(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache,
         raise ValueError('cos and sin must be contiguous FP32 on the cache\'s device')
     _check_vector(positions, 'positions', _I64, tokens, index)
     _check_vector(slots, 'slots', _I64, tokens, index)
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        raise ValueError('inference only; use torch.inference_mode()')
     out = _empty(q, (tokens, heads, dim), (heads * dim, dim, 1), dtype, index)
     if tokens:
         args = N.KV_WRITE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_weight_at, k_weight_at, cos.data_ptr(),
@@ -238,6 +244,7 @@ def read_kv(k_cache, v_cache, slots, k_scales=None, v_scales=None, dtype=None):
 
     ``dtype`` (bf16 or f16) is that of the result of an int8 cache, bf16 if not given; a 16-bit cache returns its own.
     """
+    _refuse_grad(k_cache, v_cache, k_scales, v_scales)
     call = torch.ops.kl_b200.read_kv if _traced(slots, k_cache) else read_cuda
     return call(k_cache, v_cache, slots, k_scales, v_scales, dtype)
 
@@ -275,6 +282,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     ``paged_attention_workspace_bytes``) takes the place of scratch allocated for the call; calls that share one must not
     overlap, on the device or, from several threads, on the host.
     """
+    _refuse_grad(q, k_cache, v_cache, k_scales, v_scales)
     if _traced(q, k_cache):
         both = torch.ops.kl_b200.paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales, v_scales, scale, workspace)
         return both if return_lse else both[0]
@@ -311,8 +319,6 @@ def attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_sc
         scale = dim ** -0.5
     elif not math.isfinite(scale):
         raise ValueError('scale must be finite')
-    if q.requires_grad and torch.is_grad_enabled():
-        raise ValueError('inference only; use torch.inference_mode()')
     out = _empty(q, (batch, heads, dim), (heads * dim, dim, 1), dtype, index)
     lse = _empty(q, (batch, heads), (heads, 1), _F32, index) if return_lse else None
     if batch:

@@ -222,3 +222,26 @@ def test_kv_slots_of_positions_outside_the_table():
     none = torch.zeros(2, 0, dtype=torch.int32)
     assert (kl.kv_slots(none, torch.tensor([0, 1]), torch.tensor([0, 5]), 16) < 0).all()
     assert kl.kv_slots(none, torch.tensor([], dtype=torch.int64), torch.tensor([], dtype=torch.int64), 16).shape == (0,)
+
+
+@gpu
+def test_tensors_that_require_grad_are_refused():
+    g = generator(70)
+    q, k, v, qw, kw = step_inputs(g, torch.bfloat16, 3, 4, 2, 128, True, "fused")
+    cos, sin = rope_tables(g, 128, 64)
+    at = torch.arange(3, device="cuda")
+    cache = kl.new_kv_cache(2, 16, 2, 128, torch.int8)
+    table, lengths = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    write = [q, k, v, qw, kw, cos, sin, at, at, *cache]
+    attending = [q, cache.k_cache, cache.v_cache, table, lengths, cache.k_scales, cache.v_scales]
+    reading = [cache.k_cache, cache.v_cache, at, cache.k_scales, cache.v_scales]
+    for fn, args in ((kl.qk_norm_rope_write, write), (kl.paged_attention, attending), (kl.read_kv, reading)):
+        for i, t in enumerate(args):
+            if t.is_floating_point():
+                learnt = list(args)
+                learnt[i] = torch.nn.Parameter(t.clone()) if t is qw else t.clone().requires_grad_()
+                with pytest.raises(ValueError, match="inference"):
+                    fn(*learnt)
+                with torch.no_grad():
+                    fn(*learnt)
+        fn(*args)
