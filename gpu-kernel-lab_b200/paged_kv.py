@@ -31,7 +31,6 @@ The functions are for inference: tensors that require grad are refused, as
 from __future__ import annotations
 
 import functools
-import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -54,6 +53,7 @@ _transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_st
 _BLIND = None in (_modes, _tracing, _transform)
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _I8, _I32, _I64, _F32 = torch.int8, torch.int32, torch.int64, torch.float32
+_F32_LEAST, _F32_MOST = 2.0 ** -149, 3.0e38             # what an epsilon is at least; the library's bound of both numbers
 _CODES = {torch.bfloat16: N.KL_DT_BF16, torch.float16: N.KL_DT_F16}
 
 
@@ -217,8 +217,8 @@ def write_cuda(q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache,
     if q_weight is not None and k_weight is not None:
         _check_vector(q_weight, 'q_weight', dtype, dim, index)
         _check_vector(k_weight, 'k_weight', dtype, dim, index)
-        if not 0 < epsilon < math.inf:
-            raise ValueError('epsilon must be finite and positive')
+        if not _F32_LEAST <= epsilon < _F32_MOST:
+            raise ValueError('epsilon must be finite and positive in FP32')
         q_weight_at, k_weight_at = q_weight.data_ptr(), k_weight.data_ptr()
     elif q_weight is not None or k_weight is not None:
         raise ValueError('q_weight and k_weight must be given together')
@@ -317,8 +317,8 @@ def attention_cuda(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_sc
     _check_vector(lengths, 'lengths', _I32, batch, index)
     if scale is None:
         scale = dim ** -0.5
-    elif not math.isfinite(scale):
-        raise ValueError('scale must be finite')
+    elif not -_F32_MOST < scale < _F32_MOST:
+        raise ValueError('scale must be finite in FP32')
     out = _empty(q, (batch, heads, dim), (heads * dim, dim, 1), dtype, index)
     lse = _empty(q, (batch, heads), (heads, 1), _F32, index) if return_lse else None
     if batch:

@@ -245,3 +245,17 @@ def test_tensors_that_require_grad_are_refused():
                 with torch.no_grad():
                     fn(*learnt)
         fn(*args)
+
+
+@gpu
+def test_numbers_that_f32_does_not_hold_are_refused():
+    q, cache, table, lengths = batch(generator(71), torch.bfloat16, False, 4, 2, 128, 16, [40], poison=False)
+    for scale in (1e39, -1e300, 3.39e38):
+        with pytest.raises(ValueError, match="scale"):
+            attend((q, cache, table, lengths), scale=scale)
+    qq, k, v, qw, kw = step_inputs(generator(72), torch.bfloat16, 1, 4, 2, 128, True, "fused")
+    cos, sin = rope_tables(None, 128, 8)
+    at = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for epsilon in (1e39, 1e-60, 3.39e38):
+        with pytest.raises(ValueError, match="epsilon"):
+            kl.qk_norm_rope_write(qq, k, v, qw, kw, cos, sin, at, at, *cache, epsilon=epsilon)
