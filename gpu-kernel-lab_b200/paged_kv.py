@@ -40,9 +40,9 @@ from . import _native as N
 HEAD_DIMS = (64, 128, 256)
 # A call of one token is as long as its host side, so three calls take torch's shorter ways: the current stream
 # as an integer (torch.cuda.current_stream() takes 2 us), the current device, and an allocation on it (0.9 us, 1.5 to 2.5 by
-# empty_like, new_empty or torch.empty).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
+# empty_like, new_empty or torch.empty). A torch without one of their names takes the longer way.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _empty_here = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
 _is_compiling, _is_grad_enabled = torch.compiler.is_compiling, torch.is_grad_enabled
 # Who may be looking at a call: dispatch modes (make_fx, fake tensors), jit.trace, torch.func. A torch that lacks one of these

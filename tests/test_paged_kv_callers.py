@@ -259,3 +259,33 @@ def test_numbers_that_f32_does_not_hold_are_refused():
     for epsilon in (1e39, 1e-60, 3.39e38):
         with pytest.raises(ValueError, match="epsilon"):
             kl.qk_norm_rope_write(qq, k, v, qw, kw, cos, sin, at, at, *cache, epsilon=epsilon)
+
+
+def other_torch(monkeypatch, *names):
+    """``paged_kv`` as it loads where torch lacks ``names`` of ``torch._C``."""
+    for name in names:
+        monkeypatch.delattr(torch._C, name, raising=False)
+    spec = importlib.util.spec_from_file_location(f"{kl.__name__}.paged_kv_other", ROOT / kl.__name__ / "paged_kv.py")
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+HIDDEN = ("_cuda_getCurrentRawStream", "_cuda_getDevice", "_dynamo", "_len_torch_dispatch_stack", "_is_tracing", "_functorch")
+
+
+@gpu
+@pytest.mark.parametrize("name", HIDDEN)
+def test_functions_without_torchs_private_names(monkeypatch, name):
+    case = batch(generator(73), torch.bfloat16, False, 4, 2, 128, 16, [900, 5], poison=False)
+    q, cache, table, lengths = case
+    ref = attend(case)
+    with monkeypatch.context() as m:
+        module = other_torch(m, name)
+    out = module.paged_attention(q, cache.k_cache, cache.v_cache, table, lengths)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = module.paged_attention(q, cache.k_cache, cache.v_cache, table, lengths)
+    side.synchronize()
+    assert torch.equal(out, ref) and torch.equal(again, ref)
