@@ -103,6 +103,19 @@ def test_small_weights_of_f16_caches(heads, kv_heads, dim, low, high):
     check_attention(q, cache, table, lengths, scale=math.log(2.0))
 
 
+@gpu
+def test_int8_values_of_very_different_size_for_f16_queries():
+    """A value scale of 3e7 on a key that weighs nothing."""
+    q, cache, table, lengths = batch(generator(22), torch.float16, True, 4, 2, 128, 16, [400, 90], poison=False)
+    cache.v_scales.fill_(0.01)
+    cache.v_scales[table[0, 3].long(), :, 5] = 3e7
+    cache.k_scales.fill_(0.02)
+    q = q.abs()
+    cache.k_cache.copy_(cache.k_cache.abs())
+    cache.k_cache[table[0, 3].long(), :, 5] = -127
+    check_attention(q * 2, cache, table, lengths)
+
+
 # ---- tracers -----------------------------------------------------------------------------
 def fake_step():
     """Shapes of a step, for a fake mode."""
@@ -289,3 +302,15 @@ def test_functions_without_torchs_private_names(monkeypatch, name):
         again = module.paged_attention(q, cache.k_cache, cache.v_cache, table, lengths)
     side.synchronize()
     assert torch.equal(out, ref) and torch.equal(again, ref)
+
+
+# ---- rows that are not split ---------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype,quantized", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 128), (32, 2, 128), (40, 1, 128), (16, 1, 64), (17, 1, 64), (12, 1, 256), (24, 2, 256)])
+def test_whole_rows_of_many_heads(dtype, quantized, heads, kv_heads, dim):
+    """Short rows and rows that are many are not split, with 8 and 16 heads per block and several blocks per row too."""
+    short = [n for n in LENGTHS if n <= 200]
+    check_attention(*batch(generator(heads + dim), TYPES[dtype], quantized, heads, kv_heads, dim, 16, short))
+    many = [(i * 41) % 500 if i % 7 else 0 for i in range(900 // kv_heads)] + [500]
+    check_attention(*batch(generator(heads), TYPES[dtype], quantized, heads, kv_heads, dim, 16, many))
