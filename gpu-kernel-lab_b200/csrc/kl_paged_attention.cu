@@ -262,11 +262,13 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
   if (tid == 0) {
     fence_mbar_init();
     s_piece->ways = 0;
-    prefetch_tmap(&maps.k);
-    prefetch_tmap(&maps.v);
-    if constexpr (INT8) {
-      prefetch_tmap(&maps.ks);
-      prefetch_tmap(&maps.vs);
+    if (a.box) {                                    // else there are none
+      prefetch_tmap(&maps.k);
+      prefetch_tmap(&maps.v);
+      if constexpr (INT8) {
+        prefetch_tmap(&maps.ks);
+        prefetch_tmap(&maps.vs);
+      }
     }
   }
   pdl_wait();                                       // up to here nothing was read that another kernel writes
