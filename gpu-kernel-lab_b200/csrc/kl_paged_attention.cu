@@ -837,6 +837,8 @@ __global__ void __launch_bounds__(kThreads, Geo<INT8, D, HB>::kResident)
     slot = slot + 1 == kStages ? 0 : slot + 1;
     fill = fill + 1 == kStages ? 0 : fill + 1;
   }
+  if (__any_sync(0xFFFFFFFFu, dead))                // copies still on their way are waited for once more before the memory is let go
+    for (int i = 0; i < kStages; ++i) mbar_wait_time(bar + i * 8, phases >> i & 1 ^ 1);
   if (tid == 0 && a.records) a.records[cta] = *s_piece;
 }
 
