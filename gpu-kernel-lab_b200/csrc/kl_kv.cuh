@@ -3,8 +3,8 @@
 //
 // Keys and values of one token and head are head_dim contiguous elements at
 // page * page_stride + head * head_stride + offset * token_stride, in 64-bit
-// element offsets: a cache is larger than 2^31 elements after a few hundred
-// thousand tokens.  K and V have the same strides and separate bases.
+// element offsets: a cache of 8 heads of 128 is larger than 2^31 elements
+// after two million tokens.  K and V have the same strides and separate bases.
 #pragma once
 #include "kl_common.cuh"
 

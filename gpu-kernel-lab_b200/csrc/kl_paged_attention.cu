@@ -3,9 +3,10 @@
 //   s_j = scale * q . k_j,   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   j < lengths[b]
 //
 // It is HBM-bound: every cached key and value is read once, with 4 flops per
-// element and query head. 64 int8 requests of up to 8192 tokens (16 heads on 8 of
-// 128): 108 us, 5.8 TB/s; 64 bf16 requests of 2000 tokens: 88 us, 6.0 TB/s; one bf16 request of
-// 32768 tokens: 30 us, 4.5 TB/s, of which 3 until the first copy is issued and 4 in the
+// element and query head. Replayed from a graph, 64 int8 requests of up to 8192 tokens (16 heads
+// on 8 of 128) take 108 us, 5.8 TB/s (121 us as calls under a long load, when the clock falls); 64 bf16
+// requests of 2000 tokens 88 us, 6.0 TB/s; one bf16 request of
+// 32768 tokens 30 us, 4.5 TB/s, of which 3 until the first copy is issued and 4 in the
 // join below.
 //
 // Partition. The cached tokens of a (sequence, KV head, block of query heads)
@@ -14,8 +15,8 @@
 // are only read on the device, so a captured launch serves any lengths. A row
 // that crosses CTAs leaves partial (maximum, sum, output) triples in the
 // workspace, and a dependent launch joins them in CTA order: results do not
-// depend on timing. Rows that are short, or many, are not split at all (the rule is
-// at kWholeUnits).
+// depend on timing. Rows that are short, or many, are not split at all. The host decides that
+// before it knows the lengths, by the width of the page table (the rule is at kWholeUnits).
 //
 // CTA. Four warps, each with its own keys of a unit and its own ring of kStages
 // shared-memory slots of 8 KB, filled by TMA: one box per page (or per
@@ -60,15 +61,17 @@ constexpr int kRecordBytes = 16 * 1024;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBlocks = 3;         // per SM
 constexpr int join_heads(int hb) { return hb == 16 ? 4 : 2; }   // heads of one block of the join
-// Rows of up to so many units are not split: no join, which costs 2.2 us of host time. At the most, 4 units, the
+// Rows of up to so many units, the width of the page table, are not split: no join, which costs 2.2 us of host time. At the most, 4 units, the
 // call takes 1.1 us longer on the device (8 requests of 256 tokens: 9.0 us against 7.8); with rows that are many,
 // it is shorter there too (192 f16 requests of up to 301 tokens: 19.5 against 22.3). 8 units: 14.0 us against 9.0
-// (8 requests of 500 tokens).
+// (8 requests of 500 tokens). Short rows in a table that is wide (a captured step's) are split: with 40960 tokens' columns
+// one request of 37 tokens takes 6.4 us against 5.1, 192 f16 requests of up to 301 22.5 against 19.6.
 constexpr int kWholeUnits = 4;
 // Nor are rows of up to so many units where there are two waves of rows and more: 128 requests of 1 to 500 tokens on 8
 // heads took 31.9 us against 40.5 split, of 1 to 1000 tokens 53.1 against 64.4, 256 of 1 to 2000 (32 units) 178.9 against
 // 180.2; with 1.2 waves (64 requests of 100 to 500 tokens) 23.2 against 21.4. The bound limits what one long row
-// among short ones can cost.
+// among short ones can cost. With 40960 tokens' columns these rows are split too: 128 requests of 1 to 500 tokens take 40.9 us
+// against 32.8, 256 of 1 to 250 44.0 against 32.7.
 constexpr int kWholeUnitsOfMany = 16;
 constexpr int kMaxLens = 512;          // lengths kept in shared memory
 constexpr float kSlack = 8.0f;           // log2 of how far the largest weight of a key may grow before the reference moves

@@ -19,8 +19,9 @@ codes with one f32 scale per token and head in ``k_scales`` and ``v_scales``
 turns positions into slots (``page * page_size + offset``).
 
 Arguments are checked on the host (``ValueError``).  What only the device sees
-(a position, slot, page id or length out of range) never leads to an access
-outside the buffers and is recorded for ``_native.device_status``.
+(a position, slot or page id out of range, a length beyond the page table) never leads to an
+access outside the buffers and is recorded for ``_native.device_status``; a
+negative slot is not cached and a negative length is an empty sequence.
 
 The functions are for inference: tensors that require grad are refused, as
 ``qwen_rmsnorm`` refuses them.  Called eagerly they launch directly; under
@@ -274,7 +275,8 @@ def paged_attention(q, k_cache, v_cache, page_table, lengths, k_scales=None, v_s
     * ``q`` ``[batch, heads, head_dim]``, bf16 or f16, contiguous head elements; ``heads`` a multiple of the cache's;
     * ``page_table`` int32 ``[batch, columns]``: page ``i`` of a sequence holds its tokens ``i * page_size ...``; entries
       past its length are not read;
-    * ``lengths`` int32 ``[batch]``, the new token (written before) included; a sequence of length 0 gives zeros;
+    * ``lengths`` int32 ``[batch]``, the new token (written before) included; a sequence of length 0 gives zeros; a used value
+      that is not finite makes its element infinite or NaN;
     * ``scale`` is ``head_dim ** -0.5`` if not given.
 
     Returns the output, or ``(output, lse)`` with ``return_lse``: f32 ``[batch, heads]``, the log of the sum of the

@@ -369,6 +369,8 @@ int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int to
  *   q [batch, heads, head_dim] bf16 or f16, elements contiguous; out
  *   [batch, heads, head_dim] contiguous; lse f32 [batch, heads] or NULL: the
  *   natural log of the sum of exp(scores).  lengths[b] <= 0: zeros, lse -inf.
+ *   A NaN in a used key, or a score of +inf, makes its heads' output NaN; a used value that is
+ *   not finite makes its element infinite or NaN.
  *   page_table int32 [batch, columns] by table_stride (elements).  Its entries
  *   past a sequence's length are not read.  A length beyond columns *
  *   page_size is cut to it, and keys of a page id out of range count
@@ -377,7 +379,8 @@ int kl_read_kv(const kl_kv_cache* cache, int dtype, const int64_t* slots, int to
  *   kl_paged_attention_call_bytes(...) are what one call needs, 0 (NULL allowed) where its rows
  *   are not split. 16-byte aligned.
  *   It may be kl_linear's: the first 64 KiB, which that needs zeroed, are left as
- *   they are.  Calls that share a workspace must not run concurrently.
+ *   they are.  Calls that share a workspace must not run concurrently, nor be made by several threads
+ *   at once: a split call is two launches, and nothing that uses the workspace may come between them.
  */
 size_t kl_paged_attention_workspace_bytes(int batch, int heads, int kv_heads, int head_dim);
 size_t kl_paged_attention_call_bytes(int batch, int heads, int kv_heads, int head_dim, int format, int columns, int page_size);

@@ -304,6 +304,20 @@ def test_functions_without_torchs_private_names(monkeypatch, name):
     assert torch.equal(out, ref) and torch.equal(again, ref)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_value_that_is_not_finite_stays_in_its_element(dtype):
+    case = batch(generator(74), TYPES[dtype], False, 4, 2, 128, 16, [700, 90], poison=False)
+    q, cache, table, lengths = case
+    before = attend(case)
+    for value in (torch.inf, -torch.inf, torch.nan):
+        cache.v_cache[table[0, 2].long(), 1, 5, 7] = value
+        after = attend(case)
+        hit = torch.zeros_like(before, dtype=torch.bool)
+        hit[0, 2:, 7] = True
+        assert not torch.isfinite(after[hit]).any() and torch.equal(after[~hit], before[~hit])
+
+
 # ---- rows that are not split ---------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("dtype,quantized", [("bf16", False), ("f16", False), ("bf16", True), ("f16", True)])
