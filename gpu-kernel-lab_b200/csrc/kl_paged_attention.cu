@@ -61,11 +61,11 @@ constexpr int kRecordBytes = 16 * 1024;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBlocks = 3;         // per SM
 constexpr int join_heads(int hb) { return hb == 16 ? 4 : 2; }   // heads of one block of the join
-// Rows of up to so many units, the width of the page table, are not split: no join, which costs 2.2 us of host time. At the most, 4 units, the
-// call takes 1.1 us longer on the device (8 requests of 256 tokens: 9.0 us against 7.8); with rows that are many,
-// it is shorter there too (192 f16 requests of up to 301 tokens: 19.5 against 22.3). 8 units: 14.0 us against 9.0
-// (8 requests of 500 tokens). Short rows in a table that is wide (a captured step's) are split: with 40960 tokens' columns
-// one request of 37 tokens takes 6.4 us against 5.1, 192 f16 requests of up to 301 22.5 against 19.6.
+// Rows of up to so many units (the page table's width) are not split: no join, which costs 2.2 us of host time. At the
+// most, 4 units, the call takes 1.1 us longer on the device (8 requests of 256 tokens: 9.0 us against 7.8); with rows that
+// are many, it is shorter there too (192 f16 requests of up to 301 tokens: 19.6 against 22.5). 8 units: 14.0 us against 9.0
+// (8 requests of 500 tokens). Short rows in a table that is wide (a captured step's) are split all the same: with 40960
+// tokens' columns one request of 37 tokens takes 6.4 us against 5.1, and those 192 take the 22.5.
 constexpr int kWholeUnits = 4;
 // Nor are rows of up to so many units where there are two waves of rows and more: 128 requests of 1 to 500 tokens on 8
 // heads took 31.9 us against 40.5 split, of 1 to 1000 tokens 53.1 against 64.4, 256 of 1 to 2000 (32 units) 178.9 against
